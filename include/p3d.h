@@ -241,6 +241,31 @@ int p3d_linear_headnorm(p3d_ctx *ctx, const void *x, int64_t ldx, const void *w,
                         int out_dtype, int64_t norm_cols, const float *gamma, int64_t rope_cols,
                         const float *rope_table);
 
+/* Rows to 8-bit integers (no reference counterpart): scale[i] =
+ * max(max_j |x[i][j]| / 127, 2^-126), rounded once to f32, and q[i][j] =
+ * x[i][j] / scale[i] to the nearest integer, ties to even, exactly (the
+ * result does not depend on rounding on the way).  A row holding an infinity
+ * or a NaN gets the scale NaN and zeros, so products with it are NaN.  x
+ * [m][ldx] of dtype, q [m][ldq], scale f32 [m]; columns [0, k) of q are
+ * written.  Any k and any leading dimensions >= k; rows on 16-byte boundaries
+ * are read fastest.  Quantises activations by token and weights [n][k] by
+ * output channel. */
+int p3d_quantize_rows(p3d_ctx *ctx, const void *x, int64_t ldx, int64_t m, int64_t k, int dtype, int8_t *q,
+                      int64_t ldq, float *scale);
+
+/* p3d_linear on 8-bit integers with a scale for each row of x and each output
+ * channel (no reference counterpart): y = act((sum_k x w) x_scale[row]
+ * w_scale[col] + bias), the sum exact in 32-bit integers, the rest in f32.
+ * x [m][ldx] and w [n][ldw] signed 8-bit (-128 included), 16-byte aligned,
+ * ldx and ldw multiples of 16 (k itself may be any size up to 131071; bytes
+ * from k on are not used); x_scale f32 [m], w_scale f32 [n], bias f32 [n] or
+ * NULL.  out, epilogue, gate and batch offsets as in p3d_linear; with 16-bit
+ * out GELU takes the hardware tanh, with f32 out it is accurate to f32. */
+int p3d_linear_i8(p3d_ctx *ctx, const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *w, int64_t ldw,
+                  const float *w_scale, const float *bias, int64_t m, int64_t n, int64_t k, void *out, int64_t ldo,
+                  int out_dtype, int epilogue, const float *gate, int64_t gate_ld, const int32_t *batch_offsets,
+                  int nbatch);
+
 /* Submanifold 3x3x3 sparse conv as one gather-GEMM on tcgen05 tiles:
  * out[p] = epilogue(bias + sum_k W[k] x[nbr[k][p]]).  Replaces
  * sparse_submanifold_conv3d (src/sparse.cpp:999-1055) and the ggml
@@ -295,6 +320,42 @@ int p3d_varlen_attention(p3d_ctx *ctx, const void *q, int64_t ldq, const void *k
                          const void *v, int64_t ldv, void *out, int64_t ldo, const int32_t *cu_q,
                          const int32_t *cu_k, int nseq, int64_t max_q, int64_t rows_q, int64_t rows_k,
                          int heads, int head_dim, float scale, int dtype);
+
+/* Rules of p3d_masked_attention; zeros and NULLs mean none. */
+typedef struct p3d_attention_rules {
+    float softcap;         /* > 0: scores become softcap * tanh(score / softcap) */
+    int causal;            /* nonzero: a query sees the keys up to its own position */
+    const int32_t *prefix; /* [nseq]: the first prefix[s] keys of sequence s are seen by all its queries */
+    const int32_t *doc_q;  /* [rows_q] and [rows_k], both or none: a query sees the keys of its own */
+    const int32_t *doc_k;  /*   document (equal numbers) */
+    const float *slopes;   /* [heads]: scores get -slopes[h] * |position of query - key|, after the cap */
+} p3d_attention_rules;
+
+/* Attention over packed sequences under masks and score rules (no reference
+ * counterpart: p3d_varlen_attention's operator for condition encoders, packed
+ * items and single new tokens).  Sequence s has lq = cu_q[s+1] - cu_q[s]
+ * queries and lk = cu_k[s+1] - cu_k[s] keys; query i stands at position
+ * i + lk - lq (the last query at the last key) and sees key j when
+ *   j < prefix[s], or (not causal or j <= position) and the documents agree.
+ * A query that sees no key gets zeros.  What hidden keys and rows outside the
+ * sequences hold (NaN, infinities) never reaches an output; rows of out
+ * outside the sequences are left as they were.
+ * q [rows_q][ldq], out [rows_q][ldo]: heads * head_dim columns; k, v
+ * [rows_k][ldk / ldv]: kv_heads * head_dim columns, query head h reads
+ * key/value head h / (heads / kv_heads).  head_dim 64 or 128, dtype bf16 or
+ * f16, f32 softmax and accumulation, 16-byte aligned rows.  max_q / max_k
+ * bound the queries / keys of one sequence (queries from max_q on are not
+ * computed; a max_k below the longest sequence costs time only).  The two offset arrays
+ * are device data and are clamped to the row counts.  ws:
+ * p3d_masked_attention_workspace bytes, 256-byte aligned, free again when the
+ * call's work on the stream is done (calls that may overlap need their own). */
+size_t p3d_masked_attention_workspace(int nseq, int64_t max_q, int64_t max_k, int64_t rows_q, int heads, int kv_heads,
+                                      int head_dim);
+int p3d_masked_attention(p3d_ctx *ctx, const void *q, int64_t ldq, const void *k, int64_t ldk, const void *v,
+                         int64_t ldv, void *out, int64_t ldo, const int32_t *cu_q, const int32_t *cu_k, int nseq,
+                         int64_t max_q, int64_t max_k, int64_t rows_q, int64_t rows_k, int heads, int kv_heads,
+                         int head_dim, float scale, const p3d_attention_rules *rules, void *ws, size_t ws_bytes,
+                         int dtype);
 
 /* Shifted-window sparse self-attention (no reference implementation: the
  * 8^3-window blocks of the config-3 SLat decoder).  Row i with coords
@@ -424,6 +485,22 @@ int p3d_qk_rmsnorm_rope(p3d_ctx *ctx, void *x, int64_t n, int64_t ld, int heads,
  * (1, 0). */
 int p3d_rope_table(p3d_ctx *ctx, const int32_t *coords, int64_t n, int head_dim, float freq_min,
                    float freq_base, float *table);
+
+/* Rotary positions of packed heads (no reference counterpart: the 3D RoPE
+ * above turns by voxel coordinates).  The pair (a, b) number i of every head
+ * of row r turns by the angle positions[r] * freqs[i] (64-bit):
+ * (a, b) -> amplitude * (a cos - b sin, a sin + b cos).  Pair i is elements
+ * (i, i + rot_dim / 2) of the head (P3D_ROTARY_HALF) or (2i, 2i + 1)
+ * (P3D_ROTARY_INTERLEAVED); elements from rot_dim on are copied.  x [n][ldx],
+ * out [n][ldo] of dtype (f32, bf16, f16), heads * head_dim columns; out may be
+ * x itself (same leading dimension), else they must not overlap.  positions
+ * int32 [n] or NULL for position_offset + row; freqs f64 [rot_dim / 2] on the
+ * device (plain, or stretched for long contexts by the caller).  head_dim at
+ * most 512, rot_dim even. */
+enum p3d_rotary_layout { P3D_ROTARY_HALF = 0, P3D_ROTARY_INTERLEAVED = 1 };
+int p3d_rotary(p3d_ctx *ctx, const void *x, int64_t ldx, int64_t n, int heads, int head_dim, int rot_dim, int layout,
+               const int32_t *positions, int64_t position_offset, const double *freqs, float amplitude, void *out,
+               int64_t ldo, int dtype);
 
 /* LayerNorm (+affine when gamma/beta) (+SiLU when silu != 0) written to an
  * operand of row pitch ld_out >= channels, padding columns zeroed

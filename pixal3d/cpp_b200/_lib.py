@@ -30,6 +30,9 @@ EPI_GELU_TANH = 1
 EPI_SILU = 2
 EPI_RESIDUAL = 4
 
+ROTARY_HALF = 0
+ROTARY_INTERLEAVED = 1
+
 CONV_ORDER_CHUNK_ROWS = 4096  # P3D_CONV_ORDER_CHUNK_ROWS
 
 
@@ -88,6 +91,11 @@ class ProjectionView(C.Structure):
                 ("transform_matrix", f32 * 16)]
 
 
+class AttentionRules(C.Structure):
+    """p3d_attention_rules (include/p3d.h)."""
+    _fields_ = [("softcap", f32), ("causal", i32), ("prefix", vp), ("doc_q", vp), ("doc_k", vp), ("slopes", vp)]
+
+
 class SamplerConfig(C.Structure):
     _fields_ = [("steps", i32), ("sigma_min", f32), ("rescale_t", f32), ("guidance_strength", f32),
                 ("guidance_rescale", f32), ("guidance_interval_min", f32), ("guidance_interval_max", f32),
@@ -137,6 +145,12 @@ _sig("p3d_subm_conv3d_taps", i32, vp, vp, i64, i64, vp, vp, i32, vp, i64, vp, i6
 _sig("p3d_conv_tile_taps", i32, vp, vp, i64, vp)
 _sig("p3d_varlen_attention", i32, vp, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, i32, i64, i64, i64, i32, i32, f32,
      i32)
+_sig("p3d_quantize_rows", i32, vp, vp, i64, i64, i64, i32, vp, i64, vp)
+_sig("p3d_linear_i8", i32, vp, vp, i64, vp, vp, i64, vp, vp, i64, i64, i64, vp, i64, i32, i32, vp, i64, vp, i32)
+_sig("p3d_masked_attention_workspace", sz, i32, i64, i64, i64, i32, i32, i32)
+_sig("p3d_masked_attention", i32, vp, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, i32, i64, i64, i64, i64, i32, i32, i32,
+     f32, C.POINTER(AttentionRules), vp, sz, i32)
+_sig("p3d_rotary", i32, vp, vp, i64, i64, i32, i32, i32, i32, vp, i64, vp, f32, vp, i64, i32)
 _sig("p3d_ape_add", i32, vp, vp, i64, i32, vp)
 _sig("p3d_project_features", i32, vp, C.POINTER(ProjectionView), i32, i32, vp, i64, vp, i64, i32, vp)
 _sig("p3d_projection_relative_matrices", i32, vp, vp, vp, i32, vp)

@@ -1,0 +1,107 @@
+// C ABI entry of the masked attention (kernels in p3d_masked_rows.cu).
+#include <algorithm>
+#include <cmath>
+
+#include "p3d_masked.cuh"
+
+namespace p3d {
+int masked_attention_rows(p3d_ctx *ctx, const MaskedParams &p, int head_dim, int dtype);
+
+namespace {
+
+// Blocks that fill the 148 SMs twice; a split shorter than 256 keys costs
+// more to join than it saves.
+int pick_splits(int nseq, int64_t max_q, int64_t max_k, int heads, int kv_heads) {
+    const int64_t blocks = static_cast<int64_t>(nseq) * max_q * kv_heads * ceil_div(heads / kv_heads, 16);
+    const int64_t want = ceil_div(296, std::max<int64_t>(blocks, 1));
+    return static_cast<int>(std::max<int64_t>(1, std::min({want, ceil_div(max_k, 256), int64_t(128)})));
+}
+
+size_t align256(size_t b) { return (b + 255) / 256 * 256; }
+
+}  // namespace
+}  // namespace p3d
+
+using namespace p3d;
+
+extern "C" size_t p3d_masked_attention_workspace(int nseq, int64_t max_q, int64_t max_k, int64_t rows_q, int heads,
+                                                 int kv_heads, int head_dim) {
+    if (nseq <= 0 || max_q <= 0 || max_k < 0 || rows_q <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
+    const int ns = pick_splits(nseq, max_q, max_k, heads, kv_heads);
+    if (ns == 1) return 0;
+    const size_t rows = static_cast<size_t>(rows_q) * heads * ns;
+    return align256(rows * head_dim * sizeof(float)) + align256(rows * sizeof(float2));
+}
+
+extern "C" int p3d_masked_attention(p3d_ctx *ctx, const void *q, int64_t ldq, const void *k, int64_t ldk, const void *v,
+                                    int64_t ldv, void *out, int64_t ldo, const int32_t *cu_q, const int32_t *cu_k, int nseq,
+                                    int64_t max_q, int64_t max_k, int64_t rows_q, int64_t rows_k, int heads, int kv_heads,
+                                    int head_dim, float scale, const p3d_attention_rules *rules, void *ws, size_t ws_bytes,
+                                    int dtype) {
+    if (!ctx) return P3D_ERR_INVALID;
+    P3D_REQUIRE(ctx, rows_q >= 0 && rows_k >= 0 && rows_q < (int64_t(1) << 31) && rows_k < (int64_t(1) << 31) && max_q >= 0 &&
+                         max_k >= 0 && max_q <= rows_q && max_k <= rows_k,
+                "p3d_masked_attention: bad row counts (max_q <= rows_q, max_k <= rows_k)");
+    P3D_REQUIRE(ctx, nseq > 0 && nseq < 65536, "p3d_masked_attention: bad nseq");
+    if (max_q == 0) return P3D_OK;
+    P3D_REQUIRE(ctx, q && out && cu_q && cu_k && ((k && v) || rows_k == 0), "p3d_masked_attention: null pointer");
+    if (head_dim != 64 && head_dim != 128)
+        return set_error(ctx, P3D_ERR_UNSUPPORTED, "p3d_masked_attention: head_dim must be 64 or 128");
+    P3D_REQUIRE(ctx, is_16bit(dtype), "p3d_masked_attention: dtype must be bf16 or f16");
+    P3D_REQUIRE(ctx, heads > 0 && heads < 65536 && kv_heads > 0 && heads % kv_heads == 0,
+                "p3d_masked_attention: heads must be a multiple of kv_heads");
+    P3D_REQUIRE(ctx, scale > 0.0f && std::isfinite(scale), "p3d_masked_attention: scale must be finite and positive");
+    P3D_REQUIRE(ctx, ldq % 8 == 0 && ldk % 8 == 0 && ldv % 8 == 0 && ldo % 8 == 0,
+                "p3d_masked_attention: leading dimensions must keep 16-byte rows");
+    P3D_REQUIRE(ctx, (ldq >= static_cast<int64_t>(heads) * head_dim && ldo >= static_cast<int64_t>(heads) * head_dim) || rows_q == 1,
+                "p3d_masked_attention: ldq / ldo below heads * head_dim");
+    P3D_REQUIRE(ctx, (ldk >= static_cast<int64_t>(kv_heads) * head_dim && ldv >= static_cast<int64_t>(kv_heads) * head_dim) || rows_k <= 1,
+                "p3d_masked_attention: ldk / ldv below kv_heads * head_dim");
+    P3D_REQUIRE(ctx,
+                ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+                  reinterpret_cast<uintptr_t>(out)) & 15) == 0,
+                "p3d_masked_attention: q/k/v/out must be 16-byte aligned");
+    p3d_attention_rules r{};
+    if (rules) r = *rules;
+    P3D_REQUIRE(ctx, r.softcap >= 0.0f && std::isfinite(r.softcap), "p3d_masked_attention: softcap must be finite, 0 for none");
+    P3D_REQUIRE(ctx, (r.doc_q == nullptr) == (r.doc_k == nullptr) || rows_k == 0,
+                "p3d_masked_attention: doc_q and doc_k go together");
+    const size_t need = p3d_masked_attention_workspace(nseq, max_q, max_k, rows_q, heads, kv_heads, head_dim);
+    P3D_REQUIRE(ctx, need == 0 || (ws && ws_bytes >= need && reinterpret_cast<uintptr_t>(ws) % 256 == 0),
+                "p3d_masked_attention: workspace too small or not 256-byte aligned");
+    MaskedParams p{};
+    p.q = q;
+    p.k = k;
+    p.v = v;
+    p.out = out;
+    p.ldq = ldq;
+    p.ldk = ldk;
+    p.ldv = ldv;
+    p.ldo = ldo;
+    p.cu_q = cu_q;
+    p.cu_k = cu_k;
+    p.nseq = nseq;
+    p.heads = heads;
+    p.kv_heads = kv_heads;
+    p.group = heads / kv_heads;
+    p.rows_q = rows_q;
+    p.rows_k = rows_k;
+    p.max_q = max_q;
+    constexpr float kLog2e = 1.4426950408889634f;
+    p.c0 = r.softcap > 0.0f ? scale / r.softcap * 2.0f * kLog2e : scale * kLog2e;
+    p.c1 = r.softcap > 0.0f ? r.softcap * kLog2e : 0.0f;
+    p.causal = r.causal != 0;
+    p.prefix = r.prefix;
+    p.doc_q = r.doc_q;
+    p.doc_k = r.doc_k;
+    p.slopes = r.slopes;
+    p.nsplit = pick_splits(nseq, max_q, max_k, heads, kv_heads);
+    if (p.nsplit > 1) {
+        const size_t rows = static_cast<size_t>(rows_q) * heads * p.nsplit;
+        p.part_o = static_cast<float *>(ws);
+        p.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(ws) + align256(rows * head_dim * sizeof(float)));
+    }
+    p.fault = ctx->fault;
+    DeviceGuard on(ctx->device);
+    return masked_attention_rows(ctx, p, head_dim, dtype);
+}

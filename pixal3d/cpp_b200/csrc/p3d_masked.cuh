@@ -1,0 +1,61 @@
+// What the masked-attention kernels share: the rules of visibility and of the
+// scores, and the sequence geometry.
+#pragma once
+
+#include "p3d_common.cuh"
+
+namespace p3d {
+
+struct MaskedParams {
+    const void *q, *k, *v;
+    void *out;
+    int64_t ldq, ldk, ldv, ldo;
+    const int32_t *cu_q, *cu_k;
+    int nseq, heads, kv_heads, group;
+    int64_t rows_q, rows_k, max_q;
+    // scores in units of log2: x = s c0, or with a cap x = c1 - 2 c1 / (1 + 2^(s c0))
+    float c0, c1;
+    int causal;
+    const int32_t *prefix, *doc_q, *doc_k;
+    const float *slopes;
+    int nsplit;
+    float *part_o;   // [row * heads + head][split][D]: sums against the split's own maximum
+    float2 *part_ml; // [row * heads + head][split]: (maximum, sum)
+    int *fault;
+};
+
+// Rows of sequence s.  Offsets that point outside the buffers are clamped, so
+// that a wrong offset can give a wrong result but no access out of bounds.
+struct SeqRange {
+    int q0, lq, k0, lk;
+};
+__device__ __forceinline__ SeqRange seq_range(const MaskedParams &p, int s) {
+    SeqRange r;
+    const int nq = static_cast<int>(p.rows_q), nk = static_cast<int>(p.rows_k);
+    r.q0 = min(max(p.cu_q[s], 0), nq);
+    r.lq = max(min(p.cu_q[s + 1], nq) - r.q0, 0);
+    r.k0 = min(max(p.cu_k[s], 0), nk);
+    r.lk = max(min(p.cu_k[s + 1], nk) - r.k0, 0);
+    return r;
+}
+
+__device__ __forceinline__ float ex2f(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcpf(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// The capped score in units of log2: cap log2(e) tanh(t), t = s scale / cap,
+// with tanh(t) = 1 - 2 / (1 + e^2t).  Its absolute error, some 2^-22 of the
+// cap, is what a softmax sees; the hardware tanh's 2^-11 of the score is not
+// enough (a score of 20 would be 0.01 off, 1 % of its weight).
+__device__ __forceinline__ float capped(float s, float c0, float c1) {
+    return fmaf(-2.0f * c1, rcpf(1.0f + ex2f(s * c0)), c1);
+}
+
+}  // namespace p3d

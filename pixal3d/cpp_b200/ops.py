@@ -9,6 +9,8 @@ non-zero status.  Names follow the reference's operators
 from __future__ import annotations
 
 import ctypes as C
+import math
+import threading
 
 import torch
 
@@ -28,11 +30,20 @@ class Context:
             raise P3DError(rc, f"p3d_ctx_create(device={device}) failed")
         self.h = h
         self.device = device
+        self.lock = threading.Lock()
 
     def bind(self) -> "Context":
         s = torch.cuda.current_stream(self.device).cuda_stream
         L.lib.p3d_ctx_set_stream(self.h, C.c_void_p(s))
         return self
+
+    def call(self, fn, *args) -> None:
+        """fn(ctx, *args) on torch's current stream, checked.  Threads that
+        share the context take turns, so that none launches on the stream
+        another has just bound."""
+        with self.lock:
+            L.lib.p3d_ctx_set_stream(self.h, torch._C._cuda_getCurrentRawStream(self.device))
+            self.check(fn(self.h, *args))
 
     def check(self, rc: int) -> None:
         if rc != 0:
@@ -56,6 +67,42 @@ def ctx(device: torch.device | int | None = None) -> Context:
     if idx not in _CTX:
         _CTX[idx] = Context(idx)
     return _CTX[idx].bind()
+
+
+def _ctx_of(what: str, first: torch.Tensor, *others) -> Context:
+    """The context of first's device; every other tensor has to be there too."""
+    if not first.is_cuda:
+        raise ValueError(f"{what}: tensors must be on a CUDA device")
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
+    idx = first.get_device()
+    c = _CTX.get(idx)
+    if c is None:
+        c = _CTX.setdefault(idx, Context(idx))
+    return c
+
+
+def _need(ok: bool, message: str) -> None:
+    if not ok:
+        raise ValueError(message)
+
+
+def _pitch(what: str, t: torch.Tensor, least: int) -> int:
+    """Row pitch (elements) of a 2-D view with unit column stride; of a single
+    row, `least` (its stride says nothing)."""
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise ValueError(f"{what}: expected a 2-D row-major view")
+    return t.stride(0) if t.shape[0] > 1 else least
+
+
+def _vector(what: str, t: torch.Tensor | None, n: int, dtype: torch.dtype):
+    """Pointer of a contiguous 1-D tensor of n elements, or None."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous {dtype} vector of {n}")
+    return t.data_ptr()
 
 
 def _p(t: torch.Tensor | None):
@@ -223,6 +270,64 @@ def rope_table(coords: torch.Tensor, head_dim: int = 64, freq_min: float = 1.0,
     return t
 
 
+def quantize_rows(x: torch.Tensor, out: torch.Tensor | None = None,
+                  scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """8-bit integers of rows and one f32 scale for each (p3d_quantize_rows):
+    scale = max|row| / 127, q = x / scale to the nearest, ties to even.  x
+    [m, k] f32, bf16 or f16, any row pitch.  Returns (q [m, k] int8, scale
+    [m]); a new q has rows of whole 16-byte words, as linear_i8 takes them."""
+    c = _ctx_of("quantize_rows", x, out, scale)
+    m, k = x.shape
+    _need(k > 0, "quantize_rows: rows of no elements")
+    ldx = _pitch("quantize_rows", x, k)
+    if out is None:
+        out = torch.empty((m, (k + 15) & ~15), dtype=torch.int8, device=x.device)
+        if k & 15:
+            out = out[:, :k]
+    _need(out.dtype == torch.int8 and out.shape == x.shape, "quantize_rows: out must be int8 of x's shape")
+    if scale is None:
+        scale = torch.empty(m, dtype=torch.float32, device=x.device)
+    ps = _vector("quantize_rows: scale", scale, m, torch.float32)
+    if m:
+        c.call(L.lib.p3d_quantize_rows, x.data_ptr(), ldx, m, k, _dt(x), out.data_ptr(), _pitch("quantize_rows: out", out, k),
+               ps)
+    return out, scale
+
+
+def linear_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+              bias: torch.Tensor | None = None, out: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16,
+              epilogue: int = L.EPI_NONE, gate: torch.Tensor | None = None,
+              batch_offsets: torch.Tensor | None = None) -> torch.Tensor:
+    """epilogue((x W^T) x_scale[row] w_scale[col] + b) on 8-bit integers
+    (p3d_linear_i8): x [m, k] and w [n, k] int8 as quantize_rows makes them,
+    scales and bias f32.  gate [items, n] f32 and batch_offsets as in linear."""
+    c = _ctx_of("linear_i8", x, x_scale, w, w_scale, bias, out, gate, batch_offsets)
+    m, k = x.shape
+    n = w.shape[0]
+    _need(x.dtype == torch.int8 and w.dtype == torch.int8, "linear_i8: x and w must be int8")
+    _need(w.shape[1] == k and k > 0 and n > 0, "linear_i8: x and w must have the same number of columns")
+    whole = (k + 15) & ~15
+    ldx, ldw = _pitch("linear_i8: x", x, whole), _pitch("linear_i8: w", w, whole)
+    if out is None:
+        _need(not epilogue & L.EPI_RESIDUAL, "linear_i8: the residual epilogue adds into out")
+        out = torch.empty((m, n), dtype=out_dtype, device=x.device)
+    _need(out.shape == (m, n), "linear_i8: out must be [m, n]")
+    pxs, pws = _vector("linear_i8: x_scale", x_scale, m, torch.float32), _vector("linear_i8: w_scale", w_scale, n, torch.float32)
+    pb = _vector("linear_i8: bias", bias, n, torch.float32)
+    pg = po = None
+    nb = gate_ld = 0
+    if gate is not None:
+        _need(batch_offsets is not None, "linear_i8: gate needs batch offsets")
+        nb = batch_offsets.shape[0] - 1
+        po = _vector("linear_i8: batch_offsets", batch_offsets, nb + 1, torch.int32)
+        _need(gate.dtype == torch.float32 and gate.dim() == 2 and nb > 0 and gate.shape == (nb, n), "linear_i8: gate must be f32 [items, n]")
+        pg, gate_ld = gate.data_ptr(), _pitch("linear_i8: gate", gate, n)
+    if m:
+        c.call(L.lib.p3d_linear_i8, x.data_ptr(), ldx, pxs, w.data_ptr(), ldw, pws, pb, m, n, k, out.data_ptr(),
+               _pitch("linear_i8: out", out, n), _dt(out), epilogue, pg, gate_ld, po, nb)
+    return out
+
+
 def subm_conv3d(x: torch.Tensor, nbr: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None,
                 out: torch.Tensor | None = None, out_dtype: torch.dtype = torch.float32,
                 epilogue: int = L.EPI_NONE, gate: torch.Tensor | None = None,
@@ -282,6 +387,49 @@ def varlen_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     c.check(L.lib.p3d_varlen_attention(c.h, _p(q), _rows(q), _p(k), _rows(k), _p(v), _rows(v), _p(out), _rows(out),
                                        _p(cu_q), _p(cu_k), cu_q.shape[0] - 1, max_q, q.shape[0], k.shape[0], heads,
                                        64, scale, _dt(q)))
+    return out
+
+
+def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
+                     max_q: int, max_k: int, heads: int, scale: float, kv_heads: int | None = None, causal: bool = False,
+                     prefix: torch.Tensor | None = None, doc_q: torch.Tensor | None = None,
+                     doc_k: torch.Tensor | None = None, slopes: torch.Tensor | None = None, softcap: float = 0.0,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention over packed sequences under masks and score rules
+    (p3d_masked_attention): q [rows_q, heads * d], k and v [rows_k, kv_heads *
+    d], d 64 or 128; sequence s has query rows cu_q[s]..cu_q[s+1] and key rows
+    cu_k[s]..cu_k[s+1], its last query standing at its last key.  Key j is
+    seen when j < prefix[s], or (not causal or j <= the query's position) and
+    doc_k equals doc_q; scores are softcap * tanh(score / softcap) -
+    slopes[head] * |position - j|.  A query that sees nothing gets zeros; rows
+    of a new out behind the last sequence are not written."""
+    c = _ctx_of("masked_attention", q, k, v, cu_q, cu_k, prefix, doc_q, doc_k, slopes, out)
+    _need(q.dtype in HALF and k.dtype == q.dtype and v.dtype == q.dtype, "masked_attention: q, k, v must be bf16 or f16 alike")
+    kv_heads = heads if kv_heads is None else kv_heads
+    rows_q, width = q.shape
+    rows_k = k.shape[0]
+    _need(heads > 0 and kv_heads > 0 and width % heads == 0, "masked_attention: q's columns must be heads * d")
+    d = width // heads
+    _need(k.shape == (rows_k, kv_heads * d) and v.shape == k.shape, "masked_attention: k and v must be [rows_k, kv_heads * d]")
+    nseq = cu_q.shape[0] - 1
+    pcq, pck = _vector("masked_attention: cu_q", cu_q, nseq + 1, torch.int32), _vector("masked_attention: cu_k", cu_k, nseq + 1, torch.int32)
+    if out is None:
+        out = torch.empty((rows_q, width), dtype=q.dtype, device=q.device)
+    _need(out.shape == q.shape and out.dtype == q.dtype, "masked_attention: out must be like q")
+    rules = L.AttentionRules(softcap, int(causal), _vector("masked_attention: prefix", prefix, nseq, torch.int32),
+                             _vector("masked_attention: doc_q", doc_q, rows_q, torch.int32),
+                             _vector("masked_attention: doc_k", doc_k, rows_k, torch.int32),
+                             _vector("masked_attention: slopes", slopes, heads, torch.float32))
+    _need((doc_q is None) == (doc_k is None), "masked_attention: doc_q and doc_k go together")
+    max_q, max_k = min(max_q, rows_q), min(max_k, rows_k)
+    if rows_q == 0 or nseq <= 0 or max_q <= 0:
+        return out
+    wsb = L.lib.p3d_masked_attention_workspace(nseq, max_q, max_k, rows_q, heads, kv_heads, d)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=q.device) if wsb else None
+    c.call(L.lib.p3d_masked_attention, q.data_ptr(), _pitch("masked_attention: q", q, width), k.data_ptr(),
+           _pitch("masked_attention: k", k, kv_heads * d), v.data_ptr(), _pitch("masked_attention: v", v, kv_heads * d),
+           out.data_ptr(), _pitch("masked_attention: out", out, width), pcq, pck, nseq, max_q, max_k, rows_q, rows_k, heads,
+           kv_heads, d, scale, C.byref(rules), None if ws is None else ws.data_ptr(), wsb, _dt(q))
     return out
 
 
@@ -429,6 +577,50 @@ def qk_rmsnorm_rope(x: torch.Tensor, heads: int, head_dim: int, gamma: torch.Ten
     c = ctx(x.device)
     c.check(L.lib.p3d_qk_rmsnorm_rope(c.h, _p(x), x.shape[0], _rows(x), heads, head_dim, _p(gamma), _p(coords),
                                       freq_min, freq_base, _dt(x)))
+
+
+def rotary_frequencies(rot_dim: int, base: float = 10000.0, stretch: float = 1.0, original_length: int = 4096,
+                       fast: float = 32.0, slow: float = 1.0, device=None) -> tuple[torch.Tensor, float]:
+    """(freqs, amplitude) for rotary: f64 [rot_dim / 2] angles per position,
+    base^(-2 i / rot_dim), and 1.  For contexts `stretch` > 1 times longer than
+    original_length they are interpolated by parts (the YaRN paper): a pair
+    that turns less than `slow` times within original_length is slowed by
+    `stretch`, one that turns more than `fast` times is kept, those between are
+    mixed linearly in their turns; the amplitude is 0.1 ln(stretch) + 1."""
+    _need(rot_dim >= 2 and rot_dim % 2 == 0, "rotary_frequencies: rot_dim must be even")
+    _need(base > 0 and stretch >= 1.0 and fast > slow, "rotary_frequencies: base > 0, stretch >= 1 and fast > slow wanted")
+    f = base ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
+    if stretch > 1.0:
+        keep = ((original_length * f / (2.0 * math.pi) - slow) / (fast - slow)).clamp(0.0, 1.0)
+        f = f / stretch * (1.0 - keep) + f * keep
+    return f.to(device if device is not None else "cuda"), 1.0 if stretch == 1.0 else 0.1 * math.log(stretch) + 1.0
+
+
+ROTARY_LAYOUTS = {"half": L.ROTARY_HALF, "interleaved": L.ROTARY_INTERLEAVED}
+
+
+def rotary(x: torch.Tensor, freqs: torch.Tensor, heads: int, head_dim: int, positions: torch.Tensor | None = None,
+           layout: str = "half", amplitude: float = 1.0, position_offset: int = 0,
+           out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions of the heads of x [n, heads * head_dim] (p3d_rotary):
+    pair i turns by positions[row] * freqs[i], the pair being elements (i, i +
+    rot/2) ("half") or (2i, 2i + 1) ("interleaved") with rot = 2 * len(freqs);
+    the head's other elements are copied.  positions int32, None for
+    position_offset + row.  out may be x itself."""
+    c = _ctx_of("rotary", x, freqs, positions, out)
+    _need(layout in ROTARY_LAYOUTS, "rotary: layout must be half or interleaved")
+    n, width = x.shape
+    _need(width == heads * head_dim, "rotary: x must be [n, heads * head_dim]")
+    ldx = _pitch("rotary", x, width)
+    if out is None:
+        out = torch.empty((n, width), dtype=x.dtype, device=x.device)
+    _need(out.shape == x.shape and out.dtype == x.dtype, "rotary: out must be like x")
+    half = freqs.shape[0]
+    pf, pp = _vector("rotary: freqs", freqs, half, torch.float64), _vector("rotary: positions", positions, n, torch.int32)
+    if n:
+        c.call(L.lib.p3d_rotary, x.data_ptr(), ldx, n, heads, head_dim, 2 * half, ROTARY_LAYOUTS[layout], pp, position_offset,
+               pf, amplitude, out.data_ptr(), _pitch("rotary: out", out, width), _dt(x))
+    return out
 
 
 def activation(x: torch.Tensor, act: int) -> torch.Tensor:
