@@ -69,16 +69,13 @@ def ctx(device: torch.device | int | None = None) -> Context:
     return _CTX[idx].bind()
 
 
-def _ctx_of(what: str, first: torch.Tensor, *others) -> Context:
-    """The context of first's device; every other tensor has to be there too."""
-    if not first.is_cuda:
-        raise ValueError(f"{what}: tensors must be on a CUDA device")
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
-    idx = first.get_device()
+def _ctx_on(what: str, t: torch.Tensor) -> Context:
+    """The context of t's device."""
+    idx = t.get_device()
     c = _CTX.get(idx)
     if c is None:
+        if idx < 0:
+            raise ValueError(f"{what}: tensors must be on a CUDA device")
         c = _CTX.setdefault(idx, Context(idx))
     return c
 
@@ -88,20 +85,23 @@ def _need(ok: bool, message: str) -> None:
         raise ValueError(message)
 
 
-def _pitch(what: str, t: torch.Tensor, least: int) -> int:
-    """Row pitch (elements) of a 2-D view with unit column stride; of a single
-    row, `least` (its stride says nothing)."""
-    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
-        raise ValueError(f"{what}: expected a 2-D row-major view")
-    return t.stride(0) if t.shape[0] > 1 else least
+def _matrix(what: str, t: torch.Tensor, cols: int, dtype: torch.dtype, device: int) -> int:
+    """Row pitch (elements) of a 2-D view of `cols` columns with unit column
+    stride; of a single row, `cols` (its stride says nothing)."""
+    if t.ndim != 2 or t.dtype is not dtype or t.get_device() != device or t.shape[1] != cols:
+        raise ValueError(f"{what}: expected a 2-D {dtype} tensor of {cols} columns on cuda:{device}")
+    pitch, unit = t.stride()
+    if unit != 1 and cols > 1:
+        raise ValueError(f"{what}: expected a row-major view")
+    return pitch if t.shape[0] > 1 else cols
 
 
-def _vector(what: str, t: torch.Tensor | None, n: int, dtype: torch.dtype):
+def _vector(what: str, t: torch.Tensor | None, n: int, dtype: torch.dtype, device: int):
     """Pointer of a contiguous 1-D tensor of n elements, or None."""
     if t is None:
         return None
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
-        raise ValueError(f"{what}: expected a contiguous {dtype} vector of {n}")
+    if t.dtype is not dtype or t.shape != (n,) or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous {dtype} vector of {n} on cuda:{device}")
     return t.data_ptr()
 
 
@@ -119,6 +119,7 @@ def _dt(t: torch.Tensor) -> int:
     raise TypeError(f"unsupported dtype {t.dtype}")
 
 
+_DTYPES = {torch.float32: L.P3D_F32, torch.bfloat16: L.P3D_BF16, torch.float16: L.P3D_F16}
 HALF = (torch.bfloat16, torch.float16)
 
 
@@ -276,21 +277,24 @@ def quantize_rows(x: torch.Tensor, out: torch.Tensor | None = None,
     scale = max|row| / 127, q = x / scale to the nearest, ties to even.  x
     [m, k] f32, bf16 or f16, any row pitch.  Returns (q [m, k] int8, scale
     [m]); a new q has rows of whole 16-byte words, as linear_i8 takes them."""
-    c = _ctx_of("quantize_rows", x, out, scale)
+    c = _ctx_on("quantize_rows", x)
+    dev, dt = c.device, _DTYPES.get(x.dtype)
+    if dt is None:
+        raise TypeError(f"quantize_rows: unsupported dtype {x.dtype}")
     m, k = x.shape
     _need(k > 0, "quantize_rows: rows of no elements")
-    ldx = _pitch("quantize_rows", x, k)
+    ldx = _matrix("quantize_rows", x, k, x.dtype, dev)
     if out is None:
-        out = torch.empty((m, (k + 15) & ~15), dtype=torch.int8, device=x.device)
-        if k & 15:
-            out = out[:, :k]
-    _need(out.dtype == torch.int8 and out.shape == x.shape, "quantize_rows: out must be int8 of x's shape")
+        ldq = (k + 15) & ~15
+        out = torch.empty_strided((m, k), (ldq, 1), dtype=torch.int8, device=x.device)
+    else:
+        ldq = _matrix("quantize_rows: out", out, k, torch.int8, dev)
+        _need(out.shape[0] == m, "quantize_rows: out must be of x's shape")
     if scale is None:
         scale = torch.empty(m, dtype=torch.float32, device=x.device)
-    ps = _vector("quantize_rows: scale", scale, m, torch.float32)
+    ps = _vector("quantize_rows: scale", scale, m, torch.float32, dev)
     if m:
-        c.call(L.lib.p3d_quantize_rows, x.data_ptr(), ldx, m, k, _dt(x), out.data_ptr(), _pitch("quantize_rows: out", out, k),
-               ps)
+        c.call(L.lib.p3d_quantize_rows, x.data_ptr(), ldx, m, k, dt, out.data_ptr(), ldq, ps)
     return out, scale
 
 
@@ -301,30 +305,40 @@ def linear_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     """epilogue((x W^T) x_scale[row] w_scale[col] + b) on 8-bit integers
     (p3d_linear_i8): x [m, k] and w [n, k] int8 as quantize_rows makes them,
     scales and bias f32.  gate [items, n] f32 and batch_offsets as in linear."""
-    c = _ctx_of("linear_i8", x, x_scale, w, w_scale, bias, out, gate, batch_offsets)
+    c = _ctx_on("linear_i8", x)
+    dev = c.device
     m, k = x.shape
     n = w.shape[0]
-    _need(x.dtype == torch.int8 and w.dtype == torch.int8, "linear_i8: x and w must be int8")
-    _need(w.shape[1] == k and k > 0 and n > 0, "linear_i8: x and w must have the same number of columns")
-    whole = (k + 15) & ~15
-    ldx, ldw = _pitch("linear_i8: x", x, whole), _pitch("linear_i8: w", w, whole)
+    _need(k > 0 and n > 0, "linear_i8: x or w of no elements")
+    ldx, ldw = _matrix("linear_i8: x", x, k, torch.int8, dev), _matrix("linear_i8: w", w, k, torch.int8, dev)
+    if m == 1 or n == 1:  # a lone row has no pitch; the tensor maps want one of whole 16-byte words
+        ldx, ldw = (k + 15) & ~15 if m == 1 else ldx, (k + 15) & ~15 if n == 1 else ldw
     if out is None:
         _need(not epilogue & L.EPI_RESIDUAL, "linear_i8: the residual epilogue adds into out")
-        out = torch.empty((m, n), dtype=out_dtype, device=x.device)
-    _need(out.shape == (m, n), "linear_i8: out must be [m, n]")
-    pxs, pws = _vector("linear_i8: x_scale", x_scale, m, torch.float32), _vector("linear_i8: w_scale", w_scale, n, torch.float32)
-    pb = _vector("linear_i8: bias", bias, n, torch.float32)
+        out = torch.empty(m, n, dtype=out_dtype, device=x.device)
+        ldo = n
+    else:
+        out_dtype = out.dtype
+        ldo = _matrix("linear_i8: out", out, n, out_dtype, dev)
+        _need(out.shape[0] == m, "linear_i8: out must be [m, n]")
+    dt = _DTYPES.get(out_dtype)
+    if dt is None:
+        raise TypeError(f"linear_i8: unsupported output dtype {out_dtype}")
+    pxs, pws = (_vector("linear_i8: x_scale", x_scale, m, torch.float32, dev),
+                _vector("linear_i8: w_scale", w_scale, n, torch.float32, dev))
+    pb = _vector("linear_i8: bias", bias, n, torch.float32, dev)
     pg = po = None
     nb = gate_ld = 0
     if gate is not None:
-        _need(batch_offsets is not None, "linear_i8: gate needs batch offsets")
+        _need(batch_offsets is not None and batch_offsets.shape[0] > 1, "linear_i8: gate needs batch offsets")
         nb = batch_offsets.shape[0] - 1
-        po = _vector("linear_i8: batch_offsets", batch_offsets, nb + 1, torch.int32)
-        _need(gate.dtype == torch.float32 and gate.dim() == 2 and nb > 0 and gate.shape == (nb, n), "linear_i8: gate must be f32 [items, n]")
-        pg, gate_ld = gate.data_ptr(), _pitch("linear_i8: gate", gate, n)
+        po = _vector("linear_i8: batch_offsets", batch_offsets, nb + 1, torch.int32, dev)
+        gate_ld = _matrix("linear_i8: gate", gate, n, torch.float32, dev)
+        _need(gate.shape[0] == nb, "linear_i8: gate must be [items, n]")
+        pg = gate.data_ptr()
     if m:
-        c.call(L.lib.p3d_linear_i8, x.data_ptr(), ldx, pxs, w.data_ptr(), ldw, pws, pb, m, n, k, out.data_ptr(),
-               _pitch("linear_i8: out", out, n), _dt(out), epilogue, pg, gate_ld, po, nb)
+        c.call(L.lib.p3d_linear_i8, x.data_ptr(), ldx, pxs, w.data_ptr(), ldw, pws, pb, m, n, k, out.data_ptr(), ldo, dt,
+               epilogue, pg, gate_ld, po, nb)
     return out
 
 
@@ -403,33 +417,39 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     doc_k equals doc_q; scores are softcap * tanh(score / softcap) -
     slopes[head] * |position - j|.  A query that sees nothing gets zeros; rows
     of a new out behind the last sequence are not written."""
-    c = _ctx_of("masked_attention", q, k, v, cu_q, cu_k, prefix, doc_q, doc_k, slopes, out)
-    _need(q.dtype in HALF and k.dtype == q.dtype and v.dtype == q.dtype, "masked_attention: q, k, v must be bf16 or f16 alike")
-    kv_heads = heads if kv_heads is None else kv_heads
+    c = _ctx_on("masked_attention", q)
+    dev, t, dt = c.device, q.dtype, _DTYPES.get(q.dtype)
+    _need(t is torch.bfloat16 or t is torch.float16, "masked_attention: q, k, v must be bf16 or f16")
+    if kv_heads is None:
+        kv_heads = heads
     rows_q, width = q.shape
     rows_k = k.shape[0]
     _need(heads > 0 and kv_heads > 0 and width % heads == 0, "masked_attention: q's columns must be heads * d")
     d = width // heads
-    _need(k.shape == (rows_k, kv_heads * d) and v.shape == k.shape, "masked_attention: k and v must be [rows_k, kv_heads * d]")
+    ldq = _matrix("masked_attention: q", q, width, t, dev)
+    ldk, ldv = _matrix("masked_attention: k", k, kv_heads * d, t, dev), _matrix("masked_attention: v", v, kv_heads * d, t, dev)
+    _need(v.shape[0] == rows_k, "masked_attention: k and v must have the same rows")
     nseq = cu_q.shape[0] - 1
-    pcq, pck = _vector("masked_attention: cu_q", cu_q, nseq + 1, torch.int32), _vector("masked_attention: cu_k", cu_k, nseq + 1, torch.int32)
+    pcq, pck = (_vector("masked_attention: cu_q", cu_q, nseq + 1, torch.int32, dev),
+                _vector("masked_attention: cu_k", cu_k, nseq + 1, torch.int32, dev))
     if out is None:
-        out = torch.empty((rows_q, width), dtype=q.dtype, device=q.device)
-    _need(out.shape == q.shape and out.dtype == q.dtype, "masked_attention: out must be like q")
-    rules = L.AttentionRules(softcap, int(causal), _vector("masked_attention: prefix", prefix, nseq, torch.int32),
-                             _vector("masked_attention: doc_q", doc_q, rows_q, torch.int32),
-                             _vector("masked_attention: doc_k", doc_k, rows_k, torch.int32),
-                             _vector("masked_attention: slopes", slopes, heads, torch.float32))
+        out = torch.empty(rows_q, width, dtype=t, device=q.device)
+        ldo = width
+    else:
+        ldo = _matrix("masked_attention: out", out, width, t, dev)
+        _need(out.shape[0] == rows_q, "masked_attention: out must be like q")
     _need((doc_q is None) == (doc_k is None), "masked_attention: doc_q and doc_k go together")
+    rules = L.AttentionRules(softcap, causal, _vector("masked_attention: prefix", prefix, nseq, torch.int32, dev),
+                             _vector("masked_attention: doc_q", doc_q, rows_q, torch.int32, dev),
+                             _vector("masked_attention: doc_k", doc_k, rows_k, torch.int32, dev),
+                             _vector("masked_attention: slopes", slopes, heads, torch.float32, dev))
     max_q, max_k = min(max_q, rows_q), min(max_k, rows_k)
     if rows_q == 0 or nseq <= 0 or max_q <= 0:
         return out
     wsb = L.lib.p3d_masked_attention_workspace(nseq, max_q, max_k, rows_q, heads, kv_heads, d)
     ws = torch.empty(wsb, dtype=torch.uint8, device=q.device) if wsb else None
-    c.call(L.lib.p3d_masked_attention, q.data_ptr(), _pitch("masked_attention: q", q, width), k.data_ptr(),
-           _pitch("masked_attention: k", k, kv_heads * d), v.data_ptr(), _pitch("masked_attention: v", v, kv_heads * d),
-           out.data_ptr(), _pitch("masked_attention: out", out, width), pcq, pck, nseq, max_q, max_k, rows_q, rows_k, heads,
-           kv_heads, d, scale, C.byref(rules), None if ws is None else ws.data_ptr(), wsb, _dt(q))
+    c.call(L.lib.p3d_masked_attention, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo, pcq, pck,
+           nseq, max_q, max_k, rows_q, rows_k, heads, kv_heads, d, scale, C.byref(rules), ws.data_ptr() if wsb else None, wsb, dt)
     return out
 
 
@@ -607,19 +627,27 @@ def rotary(x: torch.Tensor, freqs: torch.Tensor, heads: int, head_dim: int, posi
     rot/2) ("half") or (2i, 2i + 1) ("interleaved") with rot = 2 * len(freqs);
     the head's other elements are copied.  positions int32, None for
     position_offset + row.  out may be x itself."""
-    c = _ctx_of("rotary", x, freqs, positions, out)
-    _need(layout in ROTARY_LAYOUTS, "rotary: layout must be half or interleaved")
+    c = _ctx_on("rotary", x)
+    dev, t = c.device, x.dtype
+    dt, lay = _DTYPES.get(t), ROTARY_LAYOUTS.get(layout)
+    if dt is None:
+        raise TypeError(f"rotary: unsupported dtype {t}")
+    _need(lay is not None, "rotary: layout must be half or interleaved")
     n, width = x.shape
     _need(width == heads * head_dim, "rotary: x must be [n, heads * head_dim]")
-    ldx = _pitch("rotary", x, width)
+    ldx = _matrix("rotary", x, width, t, dev)
     if out is None:
-        out = torch.empty((n, width), dtype=x.dtype, device=x.device)
-    _need(out.shape == x.shape and out.dtype == x.dtype, "rotary: out must be like x")
+        out = torch.empty(n, width, dtype=t, device=x.device)
+        ldo = width
+    else:
+        ldo = _matrix("rotary: out", out, width, t, dev)
+        _need(out.shape[0] == n, "rotary: out must be like x")
     half = freqs.shape[0]
-    pf, pp = _vector("rotary: freqs", freqs, half, torch.float64), _vector("rotary: positions", positions, n, torch.int32)
+    pf = _vector("rotary: freqs", freqs, half, torch.float64, dev)
+    pp = _vector("rotary: positions", positions, n, torch.int32, dev)
     if n:
-        c.call(L.lib.p3d_rotary, x.data_ptr(), ldx, n, heads, head_dim, 2 * half, ROTARY_LAYOUTS[layout], pp, position_offset,
-               pf, amplitude, out.data_ptr(), _pitch("rotary: out", out, width), _dt(x))
+        c.call(L.lib.p3d_rotary, x.data_ptr(), ldx, n, heads, head_dim, 2 * half, lay, pp, position_offset, pf, amplitude,
+               out.data_ptr(), ldo, dt)
     return out
 
 
