@@ -486,6 +486,28 @@ inline size_t dtype_size(int dtype) { return dtype == P3D_F32 ? 4 : 2; }
     } while (0)
 
 // ---- misc math
+// Pairs of f32 in one register pair: one instruction for two operations.
+struct F2 {
+    unsigned long long u;
+    __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(u) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ void get(float &a, float &b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(u)); }
+};
+__device__ __forceinline__ F2 mul2(const F2 &a, const F2 &b) {
+    F2 r(0.f, 0.f);
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.u) : "l"(a.u), "l"(b.u));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(const F2 &a, const F2 &b, const F2 &c) {
+    F2 r(0.f, 0.f);
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.u) : "l"(a.u), "l"(b.u), "l"(c.u));
+    return r;
+}
+__device__ __forceinline__ F2 add2(const F2 &a, const F2 &b) {
+    F2 r(0.f, 0.f);
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.u) : "l"(a.u), "l"(b.u));
+    return r;
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

@@ -195,23 +195,6 @@ struct TileCfg {
     static_assert(TMEM == 128 || TMEM == 256 || TMEM == 512, "TMEM columns");
 };
 
-// Pairs of f32 in one register pair: one instruction for two operations.
-struct F2 {
-    unsigned long long u;
-    __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(u) : "f"(a), "f"(b)); }
-    __device__ __forceinline__ void get(float &a, float &b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(u)); }
-};
-__device__ __forceinline__ F2 mul2(const F2 &a, const F2 &b) {
-    F2 r(0.f, 0.f);
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.u) : "l"(a.u), "l"(b.u));
-    return r;
-}
-__device__ __forceinline__ F2 fma2(const F2 &a, const F2 &b, const F2 &c) {
-    F2 r(0.f, 0.f);
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.u) : "l"(a.u), "l"(b.u), "l"(c.u));
-    return r;
-}
-
 // Two values of GELU by the hardware tanh (gelu_tanh_f).
 __device__ __forceinline__ F2 gelu2(const F2 &x) {
     constexpr float c0 = 0.7978845608028654f, c1 = c0 * 0.044715f;

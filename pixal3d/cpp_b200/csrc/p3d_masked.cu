@@ -1,4 +1,5 @@
-// C ABI entry of the masked attention (kernels in p3d_masked_rows.cu).
+// C ABI entry of the masked attention (kernels in p3d_masked_rows.cu and
+// p3d_masked_fmha.cu).
 #include <algorithm>
 #include <cmath>
 
@@ -6,12 +7,17 @@
 
 namespace p3d {
 int masked_attention_rows(p3d_ctx *ctx, const MaskedParams &p, int head_dim, int dtype);
+int masked_attention_tiles(p3d_ctx *ctx, const MaskedParams &p, int head_dim, int dtype);
 
 namespace {
+
+// Up to this many queries a sequence go to the kernel that takes them one by one.
+constexpr int64_t kFewRows = 8;
 
 // Blocks that fill the 148 SMs twice; a split shorter than 256 keys costs
 // more to join than it saves.
 int pick_splits(int nseq, int64_t max_q, int64_t max_k, int heads, int kv_heads) {
+    if (max_q > kFewRows) return 1;
     const int64_t blocks = static_cast<int64_t>(nseq) * max_q * kv_heads * ceil_div(heads / kv_heads, 16);
     const int64_t want = ceil_div(296, std::max<int64_t>(blocks, 1));
     return static_cast<int>(std::max<int64_t>(1, std::min({want, ceil_div(max_k, 256), int64_t(128)})));
@@ -103,5 +109,6 @@ extern "C" int p3d_masked_attention(p3d_ctx *ctx, const void *q, int64_t ldq, co
     }
     p.fault = ctx->fault;
     DeviceGuard on(ctx->device);
-    return masked_attention_rows(ctx, p, head_dim, dtype);
+    if (max_q <= kFewRows || rows_k == 0) return masked_attention_rows(ctx, p, head_dim, dtype);
+    return masked_attention_tiles(ctx, p, head_dim, dtype);
 }

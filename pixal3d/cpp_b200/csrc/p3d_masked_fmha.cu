@@ -1,0 +1,513 @@
+// Masked attention on tcgen05 tensor cores, for many query rows.
+//
+// A CTA takes 128 queries of one head and the key blocks (64 keys) that any of
+// them sees; two CTAs share an SM (256 TMEM columns each), so one's softmax
+// runs beside the other's products.  6 warps:
+//   warp 0     finds the blocks to visit and loads them (TMA): 32 blocks are
+//              classified at a time as hidden, seen by every query, or mixed,
+//              from the positions and the documents' smallest and largest
+//              number in the block; hidden blocks are neither read nor computed
+//   warp 1     TMEM allocator, one thread issues the MMAs
+//   warps 2-5  softmax: thread = query = TMEM lane
+// Per visited block i (buffer b = i & 1): S_b = Q K^T; the softmax threads read
+// their row, apply the score rules (and, in mixed blocks only, the mask), and
+// write P_b over S_b as 16-bit; O += P_b V with P from TMEM.  The running
+// maximum is raised lazily: O and the sum are rescaled when a block's maximum
+// exceeds it by more than 8 (2^8 in P), which keeps P within 16-bit range and
+// the result exact, as both are taken against the same maximum.
+//
+// Hidden places: a hidden score is replaced by -inf whatever it was, but a
+// hidden key's V still meets P = 0 in the product, and 0 * NaN is NaN.  So the
+// V tile of a mixed block is searched for infinities and NaN before its
+// product; what is found is set to zero in shared memory and the block noted,
+// and at the end each query adds the noted blocks' non-finite values that it
+// does see.  Blocks that every query sees need none of this.
+//
+// Rows past the sequence's end compute on whatever the tile holds and are not
+// stored.  Every wait is bounded.
+#include <cstring>
+#include <type_traits>
+
+#include "p3d_masked.cuh"
+
+namespace p3d {
+namespace {
+
+constexpr int kM = 128;
+constexpr int kN = 64;
+constexpr int kThreadsF = 192;
+constexpr float kRescaleLog2 = 8.0f;
+constexpr int kSub = kN * 128;    // one 64-key x 64-dim operand tile, 128-byte rows
+constexpr int kTags = 8;          // unread tags: at most stages + 2
+constexpr uint32_t kTmemCols = 256;
+constexpr uint32_t kOCol = 128;   // S/P 0 (64) | S/P 1 (64) | O (up to 128)
+constexpr int kSmem = 100 * 1024;  // more than a third of an SM's: never a third CTA waiting for TMEM
+
+template <int D>
+struct Cfg {
+    static constexpr int SUBS = D / 64;
+    static constexpr int Q_BYTES = SUBS * kM * 128;
+    static constexpr int KV_BYTES = SUBS * kSub;
+    static constexpr int STAGES = D == 64 ? 4 : 2;  // of K, and of V
+    static_assert(Q_BYTES + 2 * STAGES * KV_BYTES + 1024 + 512 <= kSmem, "shared memory");
+    static_assert(STAGES + 2 <= kTags, "tag ring");
+};
+
+// D(tmem) (+)= A(tmem) * B(smem desc)^T, kind::f16.
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+        "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+        "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float row_max64(const float (&s)[64]) {
+    float m[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+        m[c] = fmaxf(max3f(max3f(max3f(s[c], s[8 + c], s[16 + c]), s[24 + c], s[32 + c]), s[40 + c], s[48 + c]), s[56 + c]);
+    return max3f(max3f(m[0], m[1], m[2]), max3f(m[3], m[4], m[5]), fmaxf(m[6], m[7]));
+}
+
+// Infinities and NaN of a packed pair set to zero; returns whether there were any.
+template <typename T>
+__device__ __forceinline__ bool clean_pair(uint32_t &w) {
+    constexpr uint32_t e = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+    const bool lo = (w & e) == e, hi = ((w >> 16) & e) == e;
+    if (lo) w &= 0xffff0000u;
+    if (hi) w &= 0x0000ffffu;
+    return lo || hi;
+}
+
+template <typename T, int D, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kThreadsF, 2)
+    masked_fmha_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                       const __grid_constant__ CUtensorMap tv, const MaskedParams p) {
+    using C = Cfg<D>;
+    constexpr int ST = C::STAGES;
+    pdl_wait();
+    const int head = blockIdx.x, seq = blockIdx.y;
+    const int tile = p.causal ? gridDim.z - 1 - blockIdx.z : blockIdx.z;  // the longest rows first
+    const SeqRange sr = seq_range(p, seq);
+    const int row0 = tile * kM;                       // first query of the tile, within the sequence
+    const int nrows = min(min(sr.lq, static_cast<int>(p.max_q)) - row0, kM);
+    if (nrows <= 0) return;
+    const int hk = head / p.group;
+    const int shift = sr.lk - sr.lq;                  // position of query i: i + shift
+    const int pre = p.prefix ? min(max(p.prefix[seq], 0), sr.lk) : 0;
+
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    uint8_t *sQ = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+    uint8_t *sK = sQ + C::Q_BYTES;
+    uint8_t *sV = sK + ST * C::KV_BYTES;
+    uint64_t *q_full = reinterpret_cast<uint64_t *>(sV + ST * C::KV_BYTES);
+    uint64_t *k_full = q_full + 1, *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST;
+    uint64_t *s_full = v_empty + ST, *p_full = s_full + 2, *pv_done = p_full + 2, *done_bar = pv_done + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done_bar + 1);
+    volatile int *tags = reinterpret_cast<int *>(tmem_slot + 1);  // block << 2 | mixed << 1 | last
+    int *any_seen = const_cast<int *>(tags) + kTags;
+    int *bad = any_seen + 1;  // first and last block with non-finite values taken out
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1);
+        for (int s = 0; s < ST; ++s) {
+            mbar_init(&k_full[s], 1);
+            mbar_init(&k_empty[s], 1);
+            mbar_init(&v_full[s], 1);
+            mbar_init(&v_empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&s_full[b], 1);
+            mbar_init(&p_full[b], 4);
+            mbar_init(&pv_done[b], 1);
+        }
+        mbar_init(done_bar, 1);
+        fence_barrier_init();
+        bad[0] = 0x7fffffff;
+        bad[1] = -1;
+        prefetch_tmap(&tq);
+        prefetch_tmap(&tk);
+        prefetch_tmap(&tv);
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, kTmemCols);
+        tmem_relinquish();
+    }
+
+    // Blocks to visit (warp 0, all lanes alike): bit l of `seen` / `mixed` is
+    // block chunk + l.
+    const int pos_lo = row0 + shift, pos_hi = row0 + nrows - 1 + shift;
+    const int limit = p.causal ? min(sr.lk, max(pre, pos_hi + 1)) : sr.lk;  // no query of the tile sees a key from here on
+    const int blocks = max(0, (limit + kN - 1) / kN);
+    int qdoc_lo = 0, qdoc_hi = 0;
+    int chunk = 0;
+    uint32_t seen = 0, mixed = 0;
+    auto classify = [&]() {
+        const int kb = (chunk + lane) * kN;
+        int dlo = 0, dhi = 0;
+        if (p.doc_k) {
+            // two numbers a lane and block; each block's range goes to its lane
+            const int n = min(32, blocks - chunk);
+#pragma unroll 4
+            for (int l = 0; l < n; ++l) {
+                const int j = (chunk + l) * kN + lane;
+                const int32_t *d = p.doc_k + sr.k0;
+                const int a = d[min(j, sr.lk - 1)], c = d[min(j + 32, sr.lk - 1)];
+                const int lo = __reduce_min_sync(0xffffffffu, min(a, c)), hi = __reduce_max_sync(0xffffffffu, max(a, c));
+                if (lane == l) {
+                    dlo = lo;
+                    dhi = hi;
+                }
+            }
+        }
+        const bool in = chunk + lane < blocks;
+        const bool doc_meets = !p.doc_k || (dlo <= qdoc_hi && qdoc_lo <= dhi);
+        const bool doc_all = !p.doc_k || (dlo == dhi && qdoc_lo == qdoc_hi && dlo == qdoc_lo);
+        const bool some = in && (kb < pre || doc_meets);
+        const bool all = kb + kN <= sr.lk && (kb + kN <= pre || ((!p.causal || kb + kN - 1 <= pos_lo) && doc_all));
+        seen = __ballot_sync(0xffffffffu, some);
+        mixed = __ballot_sync(0xffffffffu, some && !all);
+    };
+    auto next_block = [&](bool &is_mixed) -> int {  // the next block to visit, or -1
+        while (seen == 0) {
+            chunk += 32;
+            if (chunk >= blocks) return -1;
+            classify();
+        }
+        const int l = __ffs(seen) - 1;
+        is_mixed = (mixed >> l) & 1;
+        seen &= seen - 1;
+        return chunk + l;
+    };
+    bool cur_mixed = false;
+    int cur = -1;
+    if (warp == 0) {
+        if (p.doc_q) {
+            int lo = 0x7fffffff, hi = -0x7fffffff - 1;
+            for (int r = lane; r < nrows; r += 32) {
+                const int d = p.doc_q[sr.q0 + row0 + r];
+                lo = min(lo, d);
+                hi = max(hi, d);
+            }
+            qdoc_lo = __reduce_min_sync(0xffffffffu, lo);
+            qdoc_hi = __reduce_max_sync(0xffffffffu, hi);
+        }
+        if (blocks > 0) {
+            classify();
+            cur = next_block(cur_mixed);
+        }
+        if (lane == 0) *any_seen = cur >= 0;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    pdl_trigger();  // after the allocation: a dependent grid's CTA must not take this one's TMEM
+    const uint32_t tmem = *tmem_slot;
+    const bool nothing = *any_seen == 0;
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+
+    if (nothing) {
+        T *o = static_cast<T *>(p.out) + (sr.q0 + static_cast<int64_t>(row0)) * p.ldo + static_cast<int64_t>(head) * D;
+        for (int e = threadIdx.x; e < nrows * (D / 8); e += kThreadsF)
+            *reinterpret_cast<uint4 *>(o + (e / (D / 8)) * p.ldo + e % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
+    } else if (warp == 0) {
+        // ---------------------------------------------------------- producer
+        if (lane == 0) {
+            mbar_arrive_expect_tx(q_full, C::Q_BYTES);
+#pragma unroll
+            for (int s = 0; s < C::SUBS; ++s) tma_load_2d(sQ + s * kM * 128, &tq, q_full, head * D + s * 64, sr.q0 + row0);
+        }
+        int stage = 0;
+        uint32_t phase = 0;
+        for (int i = 0; cur >= 0; ++i) {
+            bool nxt_mixed = false;
+            const int nxt = next_block(nxt_mixed);
+            int ok = 1;
+            if (lane == 0) {
+                ok = mbar_wait(&k_empty[stage], phase ^ 1, p.fault);
+                if (ok) {
+                    tags[i % kTags] = cur << 2 | (cur_mixed ? 2 : 0) | (nxt < 0 ? 1 : 0);
+                    mbar_arrive_expect_tx(&k_full[stage], C::KV_BYTES);
+#pragma unroll
+                    for (int s = 0; s < C::SUBS; ++s)
+                        tma_load_2d(sK + stage * C::KV_BYTES + s * kSub, &tk, &k_full[stage], hk * D + s * 64, sr.k0 + cur * kN);
+                    ok = mbar_wait(&v_empty[stage], phase ^ 1, p.fault);
+                }
+                if (ok) {
+                    mbar_arrive_expect_tx(&v_full[stage], C::KV_BYTES);
+#pragma unroll
+                    for (int s = 0; s < C::SUBS; ++s)
+                        tma_load_2d(sV + stage * C::KV_BYTES + s * kSub, &tv, &v_full[stage], hk * D + s * 64, sr.k0 + cur * kN);
+                }
+            }
+            if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+            cur = nxt;
+            cur_mixed = nxt_mixed;
+            if (++stage == ST) {
+                stage = 0;
+                phase ^= 1;
+            }
+        }
+    } else if (warp == 1) {
+        // --------------------------------------------------------------- MMA
+        if (lane == 0) {
+            constexpr uint32_t idesc_s = idesc_f32acc(kM, kN, kBf16);
+            constexpr uint32_t idesc_o = idesc_f32acc(kM, D, kBf16, true);
+            const uint32_t q_addr = smem_u32(sQ);
+            bool ok = mbar_wait(q_full, 0, p.fault);
+            auto issue_pv = [&](int i) -> bool {
+                const int b = i & 1, st = i % ST;
+                if (!mbar_wait(&v_full[st], (i / ST) & 1, p.fault) || !mbar_wait(&p_full[b], (i >> 1) & 1, p.fault)) return false;
+                tc_fence_after();
+                const uint32_t v_addr = smem_u32(sV + st * C::KV_BYTES);
+#pragma unroll
+                for (int kk = 0; kk < kN / 16; ++kk)  // 16 keys: 8 packed TMEM columns of P, 2048 bytes of V
+                    umma_ts(tmem + kOCol, tmem + b * kN + kk * 8, sw128_desc_mn(v_addr + kk * 2048, kSub), idesc_o,
+                            (i > 0 || kk > 0) ? 1u : 0u);
+                umma_commit(&pv_done[b]);
+                umma_commit(&v_empty[st]);
+                return true;
+            };
+            for (int i = 0; ok; ++i) {
+                const int b = i & 1, st = i % ST;
+                if (!(ok = mbar_wait(&k_full[st], (i / ST) & 1, p.fault))) break;
+                const bool last = tags[i % kTags] & 1;
+                // S/P buffer b was last read by block i - 2's product
+                if (i >= 2 && !(ok = mbar_wait(&pv_done[b], ((i - 2) >> 1) & 1, p.fault))) break;
+                tc_fence_after();
+                const uint32_t k_addr = smem_u32(sK + st * C::KV_BYTES);
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk)
+                    umma_f16(tmem + b * kN, sw128_desc(q_addr + (kk / 4) * kM * 128 + (kk % 4) * 32),
+                             sw128_desc(k_addr + (kk / 4) * kSub + (kk % 4) * 32), idesc_s, kk > 0 ? 1u : 0u);
+                umma_commit(&s_full[b]);
+                umma_commit(&k_empty[st]);
+                if (i > 0 && !(ok = issue_pv(i - 1))) break;
+                if (last) {
+                    ok = issue_pv(i);
+                    break;
+                }
+            }
+            umma_commit(done_bar);
+            mbar_wait(done_bar, 0, p.fault);
+        }
+        __syncwarp();
+    } else {
+        // ----------------------------------------------------------- softmax
+        const int row = (warp & 3) * 32 + lane;  // TMEM lane quarter of the warp
+        const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const int pos = row0 + row + shift;
+        const bool valid = row < nrows;
+        const int docq = p.doc_q && valid ? p.doc_q[sr.q0 + row0 + row] : 0;
+        const float slope = BIAS ? p.slopes[head] * 1.4426950408889634f : 0.0f;
+        const int edge = p.causal ? min(sr.lk, max(pre, pos + 1)) : sr.lk;  // keys seen where documents do not decide
+        auto visible = [&](int j) -> bool {
+            return j < edge && (j < pre || !p.doc_k || ((!p.causal || j <= pos) && p.doc_k[sr.k0 + j] == docq));
+        };
+        float m_run = -INFINITY;
+        F2 l2(0.0f, 0.0f);
+        bool ok = true;
+        auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {  // warp-uniform: tcgen05.ld/st follow
+            int r = 1;
+            if (lane == 0) r = mbar_wait(bar, parity, p.fault) ? 1 : 0;
+            return __shfl_sync(0xffffffffu, r, 0) != 0;
+        };
+        int i = 0;
+        for (;; ++i) {
+            const int b = i & 1;
+            if (!(ok = wait(&s_full[b], (i >> 1) & 1))) break;
+            const int tag = __shfl_sync(0xffffffffu, lane == 0 ? tags[i % kTags] : 0, 0);  // lane 0 has waited
+            const int j0 = (tag >> 2) * kN;
+            tc_fence_after();
+            float s[kN];
+            {
+                float v0[32], v1[32];
+                tmem_ld32(tmem + lane_base + b * kN, v0);
+                tmem_ld32(tmem + lane_base + b * kN + 32, v1);
+                tmem_ld_wait_regs(v0);
+                tmem_ld_wait_regs(v1);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    s[e] = v0[e];
+                    s[32 + e] = v1[e];
+                }
+            }
+            if constexpr (CAP) {
+#pragma unroll
+                for (int e = 0; e < kN; ++e) s[e] = capped(s[e], p.c0, p.c1);
+            }
+            if constexpr (BIAS) {
+                const float scale = CAP ? 1.0f : p.c0;
+                const float d0 = static_cast<float>(pos - j0);
+#pragma unroll
+                for (int e = 0; e < kN; ++e) s[e] = fmaf(s[e], scale, -slope * fabsf(d0 - static_cast<float>(e)));
+            }
+            if (tag & 2) {
+                if (!p.doc_k) {
+#pragma unroll
+                    for (int e = 0; e < kN; ++e) s[e] = j0 + e < edge ? s[e] : -INFINITY;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kN; ++e) s[e] = visible(j0 + e) ? s[e] : -INFINITY;
+                }
+                // non-finite values leave the V tile before the product
+                const int st = i % ST;
+                // every lane waits: each reads what TMA wrote
+                if (!(ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], (i / ST) & 1, p.fault)))) break;
+                uint4 *v = reinterpret_cast<uint4 *>(sV + st * C::KV_BYTES);
+                bool found = false;
+                for (int e = (warp - 2) * 32 + lane; e < C::KV_BYTES / 16; e += 128) {
+                    uint4 u = v[e];
+                    bool f = clean_pair<T>(u.x);
+                    f |= clean_pair<T>(u.y);
+                    f |= clean_pair<T>(u.z);
+                    f |= clean_pair<T>(u.w);
+                    if (f) v[e] = u;
+                    found |= f;
+                }
+                if (found) {
+                    fence_proxy_async_smem();
+                    atomicMin(&bad[0], tag >> 2);
+                    atomicMax(&bad[1], tag >> 2);
+                }
+            }
+            const float unit = (CAP || BIAS) ? 1.0f : p.c0;
+            const float mx = row_max64(s) * unit;
+            const bool need = i > 0 && mx > m_run + kRescaleLog2;
+            if (i == 0) m_run = mx;
+            if (__any_sync(0xffffffffu, need)) {
+                if (!(ok = wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1))) break;
+                tc_fence_after();
+                const float alpha = need ? ex2f(m_run - mx) : 1.0f;
+                if (need) m_run = mx;
+#pragma unroll
+                for (int c = 0; c < D; c += 32) {
+                    float o[32];
+                    tmem_ld32(tmem + lane_base + kOCol + c, o);
+                    tmem_ld_wait_regs(o);
+                    uint32_t r[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(o[e] * alpha);
+                    tmem_st32(tmem + lane_base + kOCol + c, r);
+                }
+                tmem_st_wait();
+                l2 = mul2(l2, F2(alpha, alpha));
+            }
+            // a row that has seen no key yet has nothing to subtract: its weights are 2^-inf
+            const float nm = m_run == -INFINITY ? 0.0f : -m_run;
+            uint32_t pk[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+                float x0, x1;
+                fma2(F2(s[2 * e], s[2 * e + 1]), F2(unit, unit), F2(nm, nm)).get(x0, x1);
+                x0 = ex2f(x0);
+                x1 = ex2f(x1);
+                l2 = add2(l2, F2(x0, x1));
+                pk[e] = pack2<T>(x0, x1);
+            }
+            tmem_st32(tmem + lane_base + b * kN, pk);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[b]);
+            if (tag & 1) break;
+        }
+        if (ok) ok = wait(&pv_done[i & 1], (i >> 1) & 1);
+        tc_fence_after();
+        asm volatile("bar.sync 1, 128;" ::: "memory");  // every softmax warp has noted its blocks
+        float l0, l1;
+        l2.get(l0, l1);
+        const float l = l0 + l1;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const int bad0 = bad[0], bad1 = bad[1];
+        T *dst = static_cast<T *>(p.out) + (sr.q0 + static_cast<int64_t>(row0) + row) * p.ldo + static_cast<int64_t>(head) * D;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+            float o[32];
+            __syncwarp();
+            tmem_ld32(tmem + lane_base + kOCol + c, o);
+            tmem_ld_wait_regs(o);
+            if (!ok || !valid) continue;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= inv;
+            for (int j = bad0 * kN; bad1 >= 0 && j < min((bad1 + 1) * kN, sr.lk); ++j) {
+                if (!visible(j)) continue;
+                const T *v = static_cast<const T *>(p.v) + (sr.k0 + static_cast<int64_t>(j)) * p.ldv + static_cast<int64_t>(hk) * D + c;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    const float x = to_f32(v[e]);
+                    if (!isfinite(x)) o[e] += x;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+                uint4 u;
+                u.x = pack2<T>(o[e], o[e + 1]);
+                u.y = pack2<T>(o[e + 2], o[e + 3]);
+                u.z = pack2<T>(o[e + 4], o[e + 5]);
+                u.w = pack2<T>(o[e + 6], o[e + 7]);
+                *reinterpret_cast<uint4 *>(dst + c + e) = u;
+            }
+        }
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+}
+
+template <typename T, int D, bool CAP, bool BIAS>
+int launch_fmha(p3d_ctx *ctx, const MaskedParams &p, int dtype) {
+    CUtensorMap tq, tk, tv;
+    int rc = make_tmap_16bit_2d(ctx, &tq, p.q, dtype, p.rows_q, static_cast<uint64_t>(p.heads) * D, p.ldq, kM);
+    if (rc || (rc = make_tmap_16bit_2d(ctx, &tk, p.k, dtype, p.rows_k, static_cast<uint64_t>(p.kv_heads) * D, p.ldk, kN)) ||
+        (rc = make_tmap_16bit_2d(ctx, &tv, p.v, dtype, p.rows_k, static_cast<uint64_t>(p.kv_heads) * D, p.ldv, kN)))
+        return rc;
+    const int64_t tiles = ceil_div(p.max_q, kM);
+    if (tiles > 65535) return set_error(ctx, P3D_ERR_UNSUPPORTED, "p3d_masked_attention: max_q above 8388480");
+    auto kernel = masked_fmha_kernel<T, D, CAP, BIAS>;
+    P3D_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    P3D_CUDA(ctx, launch_pdl(kernel, dim3(p.heads, p.nseq, static_cast<unsigned>(tiles)), dim3(kThreadsF), kSmem, ctx->stream, tq,
+                             tk, tv, p));
+    return check_launch(ctx, "masked_fmha");
+}
+
+template <typename T, int D>
+int launch_rules(p3d_ctx *ctx, const MaskedParams &p, int dtype) {
+    if (p.c1 > 0.0f)
+        return p.slopes ? launch_fmha<T, D, true, true>(ctx, p, dtype) : launch_fmha<T, D, true, false>(ctx, p, dtype);
+    return p.slopes ? launch_fmha<T, D, false, true>(ctx, p, dtype) : launch_fmha<T, D, false, false>(ctx, p, dtype);
+}
+
+}  // namespace
+
+int masked_attention_tiles(p3d_ctx *ctx, const MaskedParams &p, int head_dim, int dtype) {
+    if (dtype == P3D_BF16)
+        return head_dim == 64 ? launch_rules<__nv_bfloat16, 64>(ctx, p, dtype) : launch_rules<__nv_bfloat16, 128>(ctx, p, dtype);
+    return head_dim == 64 ? launch_rules<__half, 64>(ctx, p, dtype) : launch_rules<__half, 128>(ctx, p, dtype);
+}
+
+}  // namespace p3d
