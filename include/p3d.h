@@ -347,10 +347,11 @@ typedef struct p3d_attention_rules {
  * bound the queries / keys of one sequence (queries from max_q on are not
  * computed; a max_k below the longest sequence costs time only).  The two offset arrays
  * are device data and are clamped to the row counts.  ws:
- * p3d_masked_attention_workspace bytes, 256-byte aligned, free again when the
+ * p3d_masked_attention_workspace bytes (documents: whether doc_q and doc_k are
+ * given), 256-byte aligned, free again when the
  * call's work on the stream is done (calls that may overlap need their own). */
-size_t p3d_masked_attention_workspace(int nseq, int64_t max_q, int64_t max_k, int64_t rows_q, int heads, int kv_heads,
-                                      int head_dim);
+size_t p3d_masked_attention_workspace(int nseq, int64_t max_q, int64_t max_k, int64_t rows_q, int64_t rows_k, int heads,
+                                      int kv_heads, int head_dim, int documents);
 int p3d_masked_attention(p3d_ctx *ctx, const void *q, int64_t ldq, const void *k, int64_t ldk, const void *v,
                          int64_t ldv, void *out, int64_t ldo, const int32_t *cu_q, const int32_t *cu_k, int nseq,
                          int64_t max_q, int64_t max_k, int64_t rows_q, int64_t rows_k, int heads, int kv_heads,

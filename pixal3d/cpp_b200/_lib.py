@@ -147,7 +147,7 @@ _sig("p3d_varlen_attention", i32, vp, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp
      i32)
 _sig("p3d_quantize_rows", i32, vp, vp, i64, i64, i64, i32, vp, i64, vp)
 _sig("p3d_linear_i8", i32, vp, vp, i64, vp, vp, i64, vp, vp, i64, i64, i64, vp, i64, i32, i32, vp, i64, vp, i32)
-_sig("p3d_masked_attention_workspace", sz, i32, i64, i64, i64, i32, i32, i32)
+_sig("p3d_masked_attention_workspace", sz, i32, i64, i64, i64, i64, i32, i32, i32, i32)
 _sig("p3d_masked_attention", i32, vp, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, i32, i64, i64, i64, i64, i32, i32, i32,
      f32, C.POINTER(AttentionRules), vp, sz, i32)
 _sig("p3d_rotary", i32, vp, vp, i64, i64, i32, i32, i32, i32, vp, i64, vp, f32, vp, i64, i32)

@@ -1,5 +1,5 @@
 // C ABI entry of the masked attention (kernels in p3d_masked_rows.cu and
-// p3d_masked_fmha.cu).
+// p3d_masked_fmha.cuh).
 #include <algorithm>
 #include <cmath>
 
@@ -7,7 +7,10 @@
 
 namespace p3d {
 int masked_attention_rows(p3d_ctx *ctx, const MaskedParams &p, int head_dim, int dtype);
-int masked_attention_tiles(p3d_ctx *ctx, const MaskedParams &p, int head_dim, int dtype);
+int masked_tiles_bf16_64(p3d_ctx *ctx, const MaskedParams &p, int dtype);
+int masked_tiles_bf16_128(p3d_ctx *ctx, const MaskedParams &p, int dtype);
+int masked_tiles_f16_64(p3d_ctx *ctx, const MaskedParams &p, int dtype);
+int masked_tiles_f16_128(p3d_ctx *ctx, const MaskedParams &p, int dtype);
 
 namespace {
 
@@ -17,10 +20,35 @@ constexpr int64_t kFewRows = 8;
 // Blocks that fill the 148 SMs twice; a split shorter than 256 keys costs
 // more to join than it saves.
 int pick_splits(int nseq, int64_t max_q, int64_t max_k, int heads, int kv_heads) {
-    if (max_q > kFewRows) return 1;
     const int64_t blocks = static_cast<int64_t>(nseq) * max_q * kv_heads * ceil_div(heads / kv_heads, 16);
     const int64_t want = ceil_div(296, std::max<int64_t>(blocks, 1));
     return static_cast<int>(std::max<int64_t>(1, std::min({want, ceil_div(max_k, 256), int64_t(128)})));
+}
+
+// Smallest and largest document number of every key block, a warp a block.
+__global__ void __launch_bounds__(256) doc_range_kernel(const MaskedParams p) {
+    pdl_wait();
+    pdl_trigger();
+    const SeqRange sr = seq_range(p, blockIdx.y);
+    const int lane = threadIdx.x & 31, step = gridDim.x * 8;
+    for (int b = blockIdx.x * 8 + (threadIdx.x >> 5); b * 64 < sr.lk; b += step) {
+        const int j = b * 64 + lane;
+        const int a = p.doc_k[sr.k0 + min(j, sr.lk - 1)], c = p.doc_k[sr.k0 + min(j + 32, sr.lk - 1)];
+        const int lo = __reduce_min_sync(0xffffffffu, min(a, c)), hi = __reduce_max_sync(0xffffffffu, max(a, c));
+        if (lane == 0) p.doc_range[doc_block(sr, blockIdx.y) + b] = make_int2(lo, hi);
+    }
+}
+
+// Many queries: the documents' block ranges, then the tensor-core kernel.
+int masked_attention_tiles(p3d_ctx *ctx, const MaskedParams &p, int head_dim, int dtype) {
+    if (p.doc_k) {
+        const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(ceil_div(std::max<int64_t>(p.max_k, 1), 8 * 64), 1024));
+        P3D_CUDA(ctx, launch_pdl(doc_range_kernel, dim3(blocks, p.nseq), dim3(256), 0, ctx->stream, p));
+        const int rc = check_launch(ctx, "doc_range");
+        if (rc) return rc;
+    }
+    if (dtype == P3D_BF16) return head_dim == 64 ? masked_tiles_bf16_64(ctx, p, dtype) : masked_tiles_bf16_128(ctx, p, dtype);
+    return head_dim == 64 ? masked_tiles_f16_64(ctx, p, dtype) : masked_tiles_f16_128(ctx, p, dtype);
 }
 
 size_t align256(size_t b) { return (b + 255) / 256 * 256; }
@@ -30,9 +58,10 @@ size_t align256(size_t b) { return (b + 255) / 256 * 256; }
 
 using namespace p3d;
 
-extern "C" size_t p3d_masked_attention_workspace(int nseq, int64_t max_q, int64_t max_k, int64_t rows_q, int heads,
-                                                 int kv_heads, int head_dim) {
-    if (nseq <= 0 || max_q <= 0 || max_k < 0 || rows_q <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
+extern "C" size_t p3d_masked_attention_workspace(int nseq, int64_t max_q, int64_t max_k, int64_t rows_q, int64_t rows_k,
+                                                 int heads, int kv_heads, int head_dim, int documents) {
+    if (nseq <= 0 || max_q <= 0 || max_k < 0 || rows_q <= 0 || rows_k < 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
+    if (max_q > kFewRows) return documents ? align256(static_cast<size_t>(rows_k / 64 + nseq + 1) * sizeof(int2)) : 0;
     const int ns = pick_splits(nseq, max_q, max_k, heads, kv_heads);
     if (ns == 1) return 0;
     const size_t rows = static_cast<size_t>(rows_q) * heads * ns;
@@ -72,7 +101,8 @@ extern "C" int p3d_masked_attention(p3d_ctx *ctx, const void *q, int64_t ldq, co
     P3D_REQUIRE(ctx, r.softcap >= 0.0f && std::isfinite(r.softcap), "p3d_masked_attention: softcap must be finite, 0 for none");
     P3D_REQUIRE(ctx, (r.doc_q == nullptr) == (r.doc_k == nullptr) || rows_k == 0,
                 "p3d_masked_attention: doc_q and doc_k go together");
-    const size_t need = p3d_masked_attention_workspace(nseq, max_q, max_k, rows_q, heads, kv_heads, head_dim);
+    const size_t need = p3d_masked_attention_workspace(nseq, max_q, max_k, rows_q, rows_k, heads, kv_heads, head_dim,
+                                                       r.doc_k != nullptr);
     P3D_REQUIRE(ctx, need == 0 || (ws && ws_bytes >= need && reinterpret_cast<uintptr_t>(ws) % 256 == 0),
                 "p3d_masked_attention: workspace too small or not 256-byte aligned");
     MaskedParams p{};
@@ -93,6 +123,7 @@ extern "C" int p3d_masked_attention(p3d_ctx *ctx, const void *q, int64_t ldq, co
     p.rows_q = rows_q;
     p.rows_k = rows_k;
     p.max_q = max_q;
+    p.max_k = max_k;
     constexpr float kLog2e = 1.4426950408889634f;
     p.c0 = r.softcap > 0.0f ? scale / r.softcap * 2.0f * kLog2e : scale * kLog2e;
     p.c1 = r.softcap > 0.0f ? r.softcap * kLog2e : 0.0f;
@@ -101,14 +132,17 @@ extern "C" int p3d_masked_attention(p3d_ctx *ctx, const void *q, int64_t ldq, co
     p.doc_q = r.doc_q;
     p.doc_k = r.doc_k;
     p.slopes = r.slopes;
+    p.fault = ctx->fault;
+    DeviceGuard on(ctx->device);
+    if (max_q > kFewRows && rows_k > 0) {
+        p.doc_range = static_cast<int2 *>(ws);
+        return masked_attention_tiles(ctx, p, head_dim, dtype);
+    }
     p.nsplit = pick_splits(nseq, max_q, max_k, heads, kv_heads);
     if (p.nsplit > 1) {
         const size_t rows = static_cast<size_t>(rows_q) * heads * p.nsplit;
         p.part_o = static_cast<float *>(ws);
         p.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(ws) + align256(rows * head_dim * sizeof(float)));
     }
-    p.fault = ctx->fault;
-    DeviceGuard on(ctx->device);
-    if (max_q <= kFewRows || rows_k == 0) return masked_attention_rows(ctx, p, head_dim, dtype);
-    return masked_attention_tiles(ctx, p, head_dim, dtype);
+    return masked_attention_rows(ctx, p, head_dim, dtype);
 }

@@ -12,7 +12,7 @@ struct MaskedParams {
     int64_t ldq, ldk, ldv, ldo;
     const int32_t *cu_q, *cu_k;
     int nseq, heads, kv_heads, group;
-    int64_t rows_q, rows_k, max_q;
+    int64_t rows_q, rows_k, max_q, max_k;
     // scores in units of log2: x = s c0, or with a cap x = c1 - 2 c1 / (1 + 2^(s c0))
     float c0, c1;
     int causal;
@@ -21,6 +21,7 @@ struct MaskedParams {
     int nsplit;
     float *part_o;   // [row * heads + head][split][D]: sums against the split's own maximum
     float2 *part_ml; // [row * heads + head][split]: (maximum, sum)
+    int2 *doc_range; // (smallest, largest) document number of every 64-key block
     int *fault;
 };
 
@@ -38,6 +39,11 @@ __device__ __forceinline__ SeqRange seq_range(const MaskedParams &p, int s) {
     r.lk = max(min(p.cu_k[s + 1], nk) - r.k0, 0);
     return r;
 }
+
+// Where the sequence's key blocks begin in doc_range: sequences that follow
+// one another never share an entry, and the last lies below
+// rows_k / 64 + nseq + 1.
+__device__ __forceinline__ int doc_block(const SeqRange &sr, int seq) { return sr.k0 / 64 + seq; }
 
 __device__ __forceinline__ float ex2f(float x) {
     float r;

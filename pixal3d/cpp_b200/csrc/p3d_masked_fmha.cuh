@@ -1,3 +1,5 @@
+#pragma once
+
 // Masked attention on tcgen05 tensor cores, for many query rows.
 //
 // A CTA takes 128 queries of one head and the key blocks (64 keys) that any of
@@ -25,7 +27,6 @@
 //
 // Rows past the sequence's end compute on whatever the tile holds and are not
 // stored.  Every wait is bounded.
-#include <cstring>
 #include <type_traits>
 
 #include "p3d_masked.cuh"
@@ -49,7 +50,7 @@ struct Cfg {
     static constexpr int Q_BYTES = SUBS * kM * 128;
     static constexpr int KV_BYTES = SUBS * kSub;
     static constexpr int STAGES = D == 64 ? 4 : 2;  // of K, and of V
-    static_assert(Q_BYTES + 2 * STAGES * KV_BYTES + 1024 + 512 <= kSmem, "shared memory");
+    static_assert(Q_BYTES + 2 * STAGES * KV_BYTES + 1024 + 512 + 4 * kN * 4 <= kSmem, "shared memory");
     static_assert(STAGES + 2 <= kTags, "tag ring");
 };
 
@@ -99,7 +100,58 @@ __device__ __forceinline__ bool clean_pair(uint32_t &w) {
     return lo || hi;
 }
 
-template <typename T, int D, bool CAP, bool BIAS>
+// Scores to capped scores in units of log2, c1 tanh(t) with t = s c0 / (2 log2
+// e).  While every t of the warp's rows is within 1/2 (scores within half the
+// cap) tanh(t) = t q(t^2), q of degree 3 fitted to an absolute error of 1.3e-7
+// (least maximum over [0, 1/2]), on the FMA pipe in pairs; otherwise by the
+// exponential and a reciprocal, which with the weights' own exponential are
+// three operations of the XU pipe for each score instead of one
+// (8192 x 8192, 16 heads of 128: XXX against YYY us).
+__device__ __forceinline__ void cap_row(float (&s)[64], float c0, float c1) {
+    constexpr float kHalfLn2 = 0.34657359027997264f;
+    const float ct = c0 * kHalfLn2;
+    float top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 64; e += 4) {
+        mul2(F2(s[e], s[e + 1]), F2(ct, ct)).get(s[e], s[e + 1]);
+        mul2(F2(s[e + 2], s[e + 3]), F2(ct, ct)).get(s[e + 2], s[e + 3]);
+        top = max3f(max3f(top, fabsf(s[e]), fabsf(s[e + 1])), fabsf(s[e + 2]), fabsf(s[e + 3]));
+    }
+    if (__all_sync(0xffffffffu, top <= 0.5f)) {
+        const float k0 = 0.999997676f * c1, k1 = -0.333206552f * c1, k2 = 0.131451456f * c1, k3 = -0.043372481f * c1;
+#pragma unroll
+        for (int e = 0; e < 64; e += 2) {
+            const F2 t(s[e], s[e + 1]);
+            const F2 u = mul2(t, t);
+            const F2 q = fma2(fma2(fma2(u, F2(k3, k3), F2(k2, k2)), u, F2(k1, k1)), u, F2(k0, k0));
+            mul2(t, q).get(s[e], s[e + 1]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 64; ++e) s[e] = capped(s[e], 2.885390081777927f, c1);
+    }
+}
+
+// s scale - slope |d - e| for the 64 keys e of a block, d the query's position
+// relative to the block's first key.  A block that lies on one side of all of
+// the warp's queries needs no absolute value.
+__device__ __forceinline__ void bias_row(float (&s)[64], float scale, float slope, int d) {
+    const float df = static_cast<float>(d);
+    const bool left = __all_sync(0xffffffffu, d >= 63), right = __all_sync(0xffffffffu, d <= 0);
+    if (left || right) {
+        const float step = left ? slope : -slope, base = -step * df;  // exact sign; one rounding, as in the other form
+#pragma unroll
+        for (int e = 0; e < 64; e += 2)
+            fma2(F2(s[e], s[e + 1]), F2(scale, scale),
+                 F2(fmaf(step, static_cast<float>(e), base), fmaf(step, static_cast<float>(e + 1), base)))
+                .get(s[e], s[e + 1]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 64; ++e) s[e] = fmaf(s[e], scale, -slope * fabsf(df - static_cast<float>(e)));
+    }
+}
+
+template <typename T, int D, bool CAP, bool BIAS, bool DOCS>
 __global__ void __launch_bounds__(kThreadsF, 2)
     masked_fmha_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                        const __grid_constant__ CUtensorMap tv, const MaskedParams p) {
@@ -128,6 +180,7 @@ __global__ void __launch_bounds__(kThreadsF, 2)
     volatile int *tags = reinterpret_cast<int *>(tmem_slot + 1);  // block << 2 | mixed << 1 | last
     int *any_seen = const_cast<int *>(tags) + kTags;
     int *bad = any_seen + 1;  // first and last block with non-finite values taken out
+    int *sdoc = reinterpret_cast<int *>((reinterpret_cast<uintptr_t>(bad + 2) + 15) & ~uintptr_t(15));  // [4 warps][64] document numbers
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -164,27 +217,23 @@ __global__ void __launch_bounds__(kThreadsF, 2)
     int qdoc_lo = 0, qdoc_hi = 0;
     int chunk = 0;
     uint32_t seen = 0, mixed = 0;
+    // The order of the visits.  Under a distance bias the scores of most rows
+    // fall away from their own position, so the tile's own block comes first,
+    // then those to its left, going away, then those to its right: the running
+    // maximum is then raised a few times and not at every block.
+    const int own_block = BIAS ? min(blocks - 1, max(0, pos_hi / kN)) : -1;
+    auto block_at = [&](int visit) { return visit <= own_block ? own_block - visit : visit; };
     auto classify = [&]() {
-        const int kb = (chunk + lane) * kN;
-        int dlo = 0, dhi = 0;
-        if (p.doc_k) {
-            // two numbers a lane and block; each block's range goes to its lane
-            const int n = min(32, blocks - chunk);
-#pragma unroll 4
-            for (int l = 0; l < n; ++l) {
-                const int j = (chunk + l) * kN + lane;
-                const int32_t *d = p.doc_k + sr.k0;
-                const int a = d[min(j, sr.lk - 1)], c = d[min(j + 32, sr.lk - 1)];
-                const int lo = __reduce_min_sync(0xffffffffu, min(a, c)), hi = __reduce_max_sync(0xffffffffu, max(a, c));
-                if (lane == l) {
-                    dlo = lo;
-                    dhi = hi;
-                }
-            }
-        }
         const bool in = chunk + lane < blocks;
-        const bool doc_meets = !p.doc_k || (dlo <= qdoc_hi && qdoc_lo <= dhi);
-        const bool doc_all = !p.doc_k || (dlo == dhi && qdoc_lo == qdoc_hi && dlo == qdoc_lo);
+        const int blk = block_at(chunk + lane), kb = blk * kN;
+        int dlo = 0, dhi = 0;
+        if (DOCS && in) {
+            const int2 r = p.doc_range[doc_block(sr, seq) + blk];
+            dlo = r.x;
+            dhi = r.y;
+        }
+        const bool doc_meets = !DOCS || (dlo <= qdoc_hi && qdoc_lo <= dhi);
+        const bool doc_all = !DOCS || (dlo == dhi && qdoc_lo == qdoc_hi && dlo == qdoc_lo);
         const bool some = in && (kb < pre || doc_meets);
         const bool all = kb + kN <= sr.lk && (kb + kN <= pre || ((!p.causal || kb + kN - 1 <= pos_lo) && doc_all));
         seen = __ballot_sync(0xffffffffu, some);
@@ -199,12 +248,12 @@ __global__ void __launch_bounds__(kThreadsF, 2)
         const int l = __ffs(seen) - 1;
         is_mixed = (mixed >> l) & 1;
         seen &= seen - 1;
-        return chunk + l;
+        return block_at(chunk + l);
     };
     bool cur_mixed = false;
     int cur = -1;
     if (warp == 0) {
-        if (p.doc_q) {
+        if (DOCS) {
             int lo = 0x7fffffff, hi = -0x7fffffff - 1;
             for (int r = lane; r < nrows; r += 32) {
                 const int d = p.doc_q[sr.q0 + row0 + r];
@@ -320,11 +369,11 @@ __global__ void __launch_bounds__(kThreadsF, 2)
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const int pos = row0 + row + shift;
         const bool valid = row < nrows;
-        const int docq = p.doc_q && valid ? p.doc_q[sr.q0 + row0 + row] : 0;
+        const int docq = DOCS && valid ? p.doc_q[sr.q0 + row0 + row] : 0;
         const float slope = BIAS ? p.slopes[head] * 1.4426950408889634f : 0.0f;
         const int edge = p.causal ? min(sr.lk, max(pre, pos + 1)) : sr.lk;  // keys seen where documents do not decide
         auto visible = [&](int j) -> bool {
-            return j < edge && (j < pre || !p.doc_k || ((!p.causal || j <= pos) && p.doc_k[sr.k0 + j] == docq));
+            return j < edge && (j < pre || !DOCS || ((!p.causal || j <= pos) && p.doc_k[sr.k0 + j] == docq));
         };
         float m_run = -INFINITY;
         F2 l2(0.0f, 0.0f);
@@ -334,47 +383,112 @@ __global__ void __launch_bounds__(kThreadsF, 2)
             if (lane == 0) r = mbar_wait(bar, parity, p.fault) ? 1 : 0;
             return __shfl_sync(0xffffffffu, r, 0) != 0;
         };
+        // documents of this warp's queries
+        const int wdoc_lo = __reduce_min_sync(0xffffffffu, valid ? docq : 0x7fffffff);
+        const int wdoc_hi = __reduce_max_sync(0xffffffffu, valid ? docq : -0x7fffffff - 1);
         int i = 0;
         for (;; ++i) {
-            const int b = i & 1;
+            const int b = i & 1, st = i % ST;
+            int tag = 0, n0 = 0, n1 = 0;
+            if constexpr (DOCS) {  // a mixed block's document numbers are on their way before its scores are there
+                if (!(ok = wait(&k_full[st], (i / ST) & 1))) break;
+                tag = __shfl_sync(0xffffffffu, lane == 0 ? tags[i % kTags] : 0, 0);  // lane 0 has waited
+                if (tag & 2) {
+                    const int j = (tag >> 2) * kN + lane;
+                    n0 = p.doc_k[sr.k0 + min(j, sr.lk - 1)];
+                    n1 = p.doc_k[sr.k0 + min(j + 32, sr.lk - 1)];
+                }
+            }
             if (!(ok = wait(&s_full[b], (i >> 1) & 1))) break;
-            const int tag = __shfl_sync(0xffffffffu, lane == 0 ? tags[i % kTags] : 0, 0);  // lane 0 has waited
+            if constexpr (!DOCS) tag = __shfl_sync(0xffffffffu, lane == 0 ? tags[i % kTags] : 0, 0);
             const int j0 = (tag >> 2) * kN;
+            bool some = true, all = !(tag & 2);  // whether this warp's queries see any key, every key of the block
+            if (DOCS && !all) {
+                const int lo = __reduce_min_sync(0xffffffffu, min(n0, n1)), hi = __reduce_max_sync(0xffffffffu, max(n0, n1));
+                some = j0 < pre || (lo <= wdoc_hi && wdoc_lo <= hi);
+                all = j0 + kN <= sr.lk && (j0 + kN <= pre || ((!p.causal || j0 + kN - 1 <= pos - lane) && lo == hi &&
+                                                               wdoc_lo == wdoc_hi && lo == wdoc_lo));
+            }
             tc_fence_after();
-            float s[kN];
-            {
-                float v0[32], v1[32];
-                tmem_ld32(tmem + lane_base + b * kN, v0);
-                tmem_ld32(tmem + lane_base + b * kN + 32, v1);
-                tmem_ld_wait_regs(v0);
-                tmem_ld_wait_regs(v1);
+            uint32_t pk[32];
+            if (some) {
+                float s[kN];
+                {
+                    float v0[32], v1[32];
+                    tmem_ld32(tmem + lane_base + b * kN, v0);
+                    tmem_ld32(tmem + lane_base + b * kN + 32, v1);
+                    tmem_ld_wait_regs(v0);
+                    tmem_ld_wait_regs(v1);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        s[e] = v0[e];
+                        s[32 + e] = v1[e];
+                    }
+                }
+                if constexpr (CAP) cap_row(s, p.c0, p.c1);
+                if constexpr (BIAS) bias_row(s, CAP ? 1.0f : p.c0, slope, pos - j0);
+                if (!all) {
+                    if constexpr (!DOCS) {
+#pragma unroll
+                        for (int e = 0; e < kN; ++e) s[e] = j0 + e < edge ? s[e] : -INFINITY;
+                    } else {
+                        int *d = sdoc + (warp - 2) * kN;
+                        __syncwarp();
+                        d[lane] = n0;
+                        d[lane + 32] = n1;
+                        __syncwarp();
+                        // (bitwise: short-circuit forms became 64 divergent branches, 4.4 us a block)
+                        const int own = (p.causal ? min(sr.lk, pos + 1) : sr.lk) - j0, shared = pre - j0;
+#pragma unroll
+                        for (int e = 0; e < kN; e += 4) {
+                            const int4 n = *reinterpret_cast<const int4 *>(d + e);
+                            s[e] = ((e < shared) | ((e < own) & (n.x == docq))) ? s[e] : -INFINITY;
+                            s[e + 1] = ((e + 1 < shared) | ((e + 1 < own) & (n.y == docq))) ? s[e + 1] : -INFINITY;
+                            s[e + 2] = ((e + 2 < shared) | ((e + 2 < own) & (n.z == docq))) ? s[e + 2] : -INFINITY;
+                            s[e + 3] = ((e + 3 < shared) | ((e + 3 < own) & (n.w == docq))) ? s[e + 3] : -INFINITY;
+                        }
+                    }
+                }
+                const float unit = (CAP || BIAS) ? 1.0f : p.c0;
+                const float mx = row_max64(s) * unit;
+                const bool need = i > 0 && mx > m_run + kRescaleLog2;
+                if (i == 0) m_run = mx;
+                if (__any_sync(0xffffffffu, need)) {
+                    if (!(ok = wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1))) break;
+                    tc_fence_after();
+                    const float alpha = need ? ex2f(m_run - mx) : 1.0f;
+                    if (need) m_run = mx;
+#pragma unroll
+                    for (int c = 0; c < D; c += 32) {
+                        float o[32];
+                        tmem_ld32(tmem + lane_base + kOCol + c, o);
+                        tmem_ld_wait_regs(o);
+                        uint32_t r[32];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(o[e] * alpha);
+                        tmem_st32(tmem + lane_base + kOCol + c, r);
+                    }
+                    tmem_st_wait();
+                    l2 = mul2(l2, F2(alpha, alpha));
+                }
+                // a row that has seen no key yet has nothing to subtract: its weights are 2^-inf
+                const float nm = m_run == -INFINITY ? 0.0f : -m_run;
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
-                    s[e] = v0[e];
-                    s[32 + e] = v1[e];
+                    float x0, x1;
+                    fma2(F2(s[2 * e], s[2 * e + 1]), F2(unit, unit), F2(nm, nm)).get(x0, x1);
+                    x0 = ex2f(x0);
+                    x1 = ex2f(x1);
+                    l2 = add2(l2, F2(x0, x1));
+                    pk[e] = pack2<T>(x0, x1);
                 }
-            }
-            if constexpr (CAP) {
+            } else {
 #pragma unroll
-                for (int e = 0; e < kN; ++e) s[e] = capped(s[e], p.c0, p.c1);
-            }
-            if constexpr (BIAS) {
-                const float scale = CAP ? 1.0f : p.c0;
-                const float d0 = static_cast<float>(pos - j0);
-#pragma unroll
-                for (int e = 0; e < kN; ++e) s[e] = fmaf(s[e], scale, -slope * fabsf(d0 - static_cast<float>(e)));
+                for (int e = 0; e < 32; ++e) pk[e] = 0;
             }
             if (tag & 2) {
-                if (!p.doc_k) {
-#pragma unroll
-                    for (int e = 0; e < kN; ++e) s[e] = j0 + e < edge ? s[e] : -INFINITY;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < kN; ++e) s[e] = visible(j0 + e) ? s[e] : -INFINITY;
-                }
-                // non-finite values leave the V tile before the product
-                const int st = i % ST;
-                // every lane waits: each reads what TMA wrote
+                // non-finite values leave the V tile before the product; every
+                // lane waits, as each reads what TMA wrote
                 if (!(ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], (i / ST) & 1, p.fault)))) break;
                 uint4 *v = reinterpret_cast<uint4 *>(sV + st * C::KV_BYTES);
                 bool found = false;
@@ -392,40 +506,7 @@ __global__ void __launch_bounds__(kThreadsF, 2)
                     atomicMin(&bad[0], tag >> 2);
                     atomicMax(&bad[1], tag >> 2);
                 }
-            }
-            const float unit = (CAP || BIAS) ? 1.0f : p.c0;
-            const float mx = row_max64(s) * unit;
-            const bool need = i > 0 && mx > m_run + kRescaleLog2;
-            if (i == 0) m_run = mx;
-            if (__any_sync(0xffffffffu, need)) {
-                if (!(ok = wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1))) break;
-                tc_fence_after();
-                const float alpha = need ? ex2f(m_run - mx) : 1.0f;
-                if (need) m_run = mx;
-#pragma unroll
-                for (int c = 0; c < D; c += 32) {
-                    float o[32];
-                    tmem_ld32(tmem + lane_base + kOCol + c, o);
-                    tmem_ld_wait_regs(o);
-                    uint32_t r[32];
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(o[e] * alpha);
-                    tmem_st32(tmem + lane_base + kOCol + c, r);
-                }
-                tmem_st_wait();
-                l2 = mul2(l2, F2(alpha, alpha));
-            }
-            // a row that has seen no key yet has nothing to subtract: its weights are 2^-inf
-            const float nm = m_run == -INFINITY ? 0.0f : -m_run;
-            uint32_t pk[32];
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-                float x0, x1;
-                fma2(F2(s[2 * e], s[2 * e + 1]), F2(unit, unit), F2(nm, nm)).get(x0, x1);
-                x0 = ex2f(x0);
-                x1 = ex2f(x1);
-                l2 = add2(l2, F2(x0, x1));
-                pk[e] = pack2<T>(x0, x1);
+                __syncwarp();
             }
             tmem_st32(tmem + lane_base + b * kN, pk);
             tmem_st_wait();
@@ -479,7 +560,7 @@ __global__ void __launch_bounds__(kThreadsF, 2)
     if (warp == 1) tmem_dealloc(tmem, kTmemCols);
 }
 
-template <typename T, int D, bool CAP, bool BIAS>
+template <typename T, int D, bool CAP, bool BIAS, bool DOCS>
 int launch_fmha(p3d_ctx *ctx, const MaskedParams &p, int dtype) {
     CUtensorMap tq, tk, tv;
     int rc = make_tmap_16bit_2d(ctx, &tq, p.q, dtype, p.rows_q, static_cast<uint64_t>(p.heads) * D, p.ldq, kM);
@@ -488,26 +569,25 @@ int launch_fmha(p3d_ctx *ctx, const MaskedParams &p, int dtype) {
         return rc;
     const int64_t tiles = ceil_div(p.max_q, kM);
     if (tiles > 65535) return set_error(ctx, P3D_ERR_UNSUPPORTED, "p3d_masked_attention: max_q above 8388480");
-    auto kernel = masked_fmha_kernel<T, D, CAP, BIAS>;
+    auto kernel = masked_fmha_kernel<T, D, CAP, BIAS, DOCS>;
     P3D_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     P3D_CUDA(ctx, launch_pdl(kernel, dim3(p.heads, p.nseq, static_cast<unsigned>(tiles)), dim3(kThreadsF), kSmem, ctx->stream, tq,
                              tk, tv, p));
     return check_launch(ctx, "masked_fmha");
 }
 
-template <typename T, int D>
+template <typename T, int D, bool DOCS>
 int launch_rules(p3d_ctx *ctx, const MaskedParams &p, int dtype) {
     if (p.c1 > 0.0f)
-        return p.slopes ? launch_fmha<T, D, true, true>(ctx, p, dtype) : launch_fmha<T, D, true, false>(ctx, p, dtype);
-    return p.slopes ? launch_fmha<T, D, false, true>(ctx, p, dtype) : launch_fmha<T, D, false, false>(ctx, p, dtype);
+        return p.slopes ? launch_fmha<T, D, true, true, DOCS>(ctx, p, dtype) : launch_fmha<T, D, true, false, DOCS>(ctx, p, dtype);
+    return p.slopes ? launch_fmha<T, D, false, true, DOCS>(ctx, p, dtype) : launch_fmha<T, D, false, false, DOCS>(ctx, p, dtype);
+}
+
+// The kernel of a type, head_dim and rules (one translation unit a type and head_dim).
+template <typename T, int D>
+int masked_tiles(p3d_ctx *ctx, const MaskedParams &p, int dtype) {
+    return p.doc_k ? launch_rules<T, D, true>(ctx, p, dtype) : launch_rules<T, D, false>(ctx, p, dtype);
 }
 
 }  // namespace
-
-int masked_attention_tiles(p3d_ctx *ctx, const MaskedParams &p, int head_dim, int dtype) {
-    if (dtype == P3D_BF16)
-        return head_dim == 64 ? launch_rules<__nv_bfloat16, 64>(ctx, p, dtype) : launch_rules<__nv_bfloat16, 128>(ctx, p, dtype);
-    return head_dim == 64 ? launch_rules<__half, 64>(ctx, p, dtype) : launch_rules<__half, 128>(ctx, p, dtype);
-}
-
 }  // namespace p3d

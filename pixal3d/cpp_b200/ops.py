@@ -446,7 +446,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     max_q, max_k = min(max_q, rows_q), min(max_k, rows_k)
     if rows_q == 0 or nseq <= 0 or max_q <= 0:
         return out
-    wsb = L.lib.p3d_masked_attention_workspace(nseq, max_q, max_k, rows_q, heads, kv_heads, d)
+    wsb = L.lib.p3d_masked_attention_workspace(nseq, max_q, max_k, rows_q, rows_k, heads, kv_heads, d, doc_k is not None)
     ws = torch.empty(wsb, dtype=torch.uint8, device=q.device) if wsb else None
     c.call(L.lib.p3d_masked_attention, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo, pcq, pck,
            nseq, max_q, max_k, rows_q, rows_k, heads, kv_heads, d, scale, C.byref(rules), ws.data_ptr() if wsb else None, wsb, dt)

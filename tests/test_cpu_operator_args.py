@@ -29,9 +29,12 @@ def test_null_context_is_refused():
 
 def test_masked_attention_workspace():
     ws = L.lib.p3d_masked_attention_workspace
-    assert ws(0, 1, 1, 1, 1, 1, 64) == 0 and ws(1, 0, 1, 1, 1, 1, 64) == 0
-    assert ws(1, 1, 16384, 1, 16, 4, 128) >= 2 * 16 * 128 * 4  # one token over a long cache: split keys
-    assert ws(1, 1, 16384, 1, 16, 4, 128) <= ws(1, 1, 65536, 1, 16, 4, 128)
+    assert ws(0, 1, 1, 1, 1, 1, 1, 64, 0) == 0 and ws(1, 0, 1, 1, 1, 1, 1, 64, 0) == 0
+    token = ws(1, 1, 16384, 1, 16384, 16, 4, 128, 0)
+    assert token >= 2 * 16 * 128 * 4  # one token over a long cache: its keys are split
+    assert token <= ws(1, 1, 65536, 1, 65536, 16, 4, 128, 0)
+    assert ws(3, 500, 500, 1500, 1500, 16, 4, 128, 0) == 0
+    assert ws(3, 500, 500, 1500, 1500, 16, 4, 128, 1) >= 8 * (1500 // 64 + 3 + 1)  # a range for every block of keys
 
 
 def test_rotary_frequencies_on_the_host():
