@@ -7,6 +7,8 @@
 
 namespace p3d {
 int masked_attention_rows(p3d_ctx *ctx, const MaskedParams &p, int head_dim, int dtype);
+// Ranges that the key tiles of `items` items are cut into, 0 for a block an item.
+int masked_rows_ranges(int64_t items, int64_t max_k, int group, int head_dim);
 int masked_tiles_bf16_64(p3d_ctx *ctx, const MaskedParams &p, int dtype);
 int masked_tiles_bf16_128(p3d_ctx *ctx, const MaskedParams &p, int dtype);
 int masked_tiles_f16_64(p3d_ctx *ctx, const MaskedParams &p, int dtype);
@@ -16,14 +18,6 @@ namespace {
 
 // Up to this many queries a sequence go to the kernel that takes them one by one.
 constexpr int64_t kFewRows = 8;
-
-// Blocks that fill the 148 SMs twice; a split shorter than 256 keys costs
-// more to join than it saves.
-int pick_splits(int nseq, int64_t max_q, int64_t max_k, int heads, int kv_heads) {
-    const int64_t blocks = static_cast<int64_t>(nseq) * max_q * kv_heads * ceil_div(heads / kv_heads, 16);
-    const int64_t want = ceil_div(296, std::max<int64_t>(blocks, 1));
-    return static_cast<int>(std::max<int64_t>(1, std::min({want, ceil_div(max_k, 256), int64_t(128)})));
-}
 
 // Smallest and largest document number of every key block, a warp a block.
 __global__ void __launch_bounds__(256) doc_range_kernel(const MaskedParams p) {
@@ -53,6 +47,17 @@ int masked_attention_tiles(p3d_ctx *ctx, const MaskedParams &p, int head_dim, in
 
 size_t align256(size_t b) { return (b + 255) / 256 * 256; }
 
+// Ranges of the rows kernel and the bytes of its parts' sums and (maximum, sum).
+int rows_parts(int nseq, int64_t max_q, int64_t max_k, int heads, int kv_heads, int head_dim, size_t &o, size_t &ml) {
+    const int group = heads / kv_heads, per = group > 8 ? 16 : 8;
+    const int64_t items = static_cast<int64_t>(nseq) * max_q * kv_heads * ceil_div(group, per);
+    const int ranges = masked_rows_ranges(items, max_k, group, head_dim);
+    const size_t parts = static_cast<size_t>(ranges + items) * per;
+    o = align256(parts * head_dim * sizeof(float));
+    ml = align256(parts * sizeof(float2));
+    return ranges;
+}
+
 }  // namespace
 }  // namespace p3d
 
@@ -62,10 +67,8 @@ extern "C" size_t p3d_masked_attention_workspace(int nseq, int64_t max_q, int64_
                                                  int heads, int kv_heads, int head_dim, int documents) {
     if (nseq <= 0 || max_q <= 0 || max_k < 0 || rows_q <= 0 || rows_k < 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
     if (max_q > kFewRows) return documents ? align256(static_cast<size_t>(rows_k / 64 + nseq + 1) * sizeof(int2)) : 0;
-    const int ns = pick_splits(nseq, max_q, max_k, heads, kv_heads);
-    if (ns == 1) return 0;
-    const size_t rows = static_cast<size_t>(rows_q) * heads * ns;
-    return align256(rows * head_dim * sizeof(float)) + align256(rows * sizeof(float2));
+    size_t o, ml;
+    return rows_parts(nseq, max_q, max_k, heads, kv_heads, head_dim, o, ml) ? o + ml : 0;
 }
 
 extern "C" int p3d_masked_attention(p3d_ctx *ctx, const void *q, int64_t ldq, const void *k, int64_t ldk, const void *v,
@@ -138,11 +141,10 @@ extern "C" int p3d_masked_attention(p3d_ctx *ctx, const void *q, int64_t ldq, co
         p.doc_range = static_cast<int2 *>(ws);
         return masked_attention_tiles(ctx, p, head_dim, dtype);
     }
-    p.nsplit = pick_splits(nseq, max_q, max_k, heads, kv_heads);
-    if (p.nsplit > 1) {
-        const size_t rows = static_cast<size_t>(rows_q) * heads * p.nsplit;
-        p.part_o = static_cast<float *>(ws);
-        p.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(ws) + align256(rows * head_dim * sizeof(float)));
-    }
+    size_t o, ml;
+    p.head_tiles = static_cast<int>(ceil_div(p.group, p.group > 8 ? 16 : 8));
+    p.ranges = rows_parts(nseq, max_q, max_k, heads, kv_heads, head_dim, o, ml);
+    p.part_o = static_cast<float *>(ws);
+    p.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(ws) + o);
     return masked_attention_rows(ctx, p, head_dim, dtype);
 }

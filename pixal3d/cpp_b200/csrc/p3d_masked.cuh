@@ -18,9 +18,12 @@ struct MaskedParams {
     int causal;
     const int32_t *prefix, *doc_q, *doc_k;
     const float *slopes;
-    int nsplit;
-    float *part_o;   // [row * heads + head][split][D]: sums against the split's own maximum
-    float2 *part_ml; // [row * heads + head][split]: (maximum, sum)
+    // the rows kernel: groups of 8 or 16 heads of a K/V head; equal ranges the
+    // key tiles are cut into (0: a block an item), and the parts' sums [part]
+    // [8 or 16 heads][D] against their own maxima, [part][heads] (maximum, sum)
+    int head_tiles, ranges;
+    float *part_o;
+    float2 *part_ml;
     int2 *doc_range; // (smallest, largest) document number of every 64-key block
     int *fault;
 };
