@@ -7,7 +7,8 @@ Every .cu under csrc/ is compiled with
 into _build/*.o (parallel, incremental on source/header mtimes) and linked
 into pixal3d/cpp_b200/libp3dcuda.so with a static CUDA runtime.  The C++17
 host layer (host/*.cpp: the reference's include/pixal3d API on top of the
-C ABI) is linked into libpixal3d_b200.so next to it.
+C ABI) is linked into libpixal3d_b200.so next to it, and the native torch
+binding (bind/p3d_bind.cpp, against the installed torch's headers) into _bind.so.
 """
 from __future__ import annotations
 
@@ -26,6 +27,8 @@ HOST = PKG / "host"
 BUILD = PKG / "_build"
 LIB = PKG / "libp3dcuda.so"
 HOST_LIB = PKG / "libpixal3d_b200.so"
+BIND = PKG / "bind" / "p3d_bind.cpp"
+BIND_LIB = PKG / "_bind.so"
 INCLUDE = REPO / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -91,7 +94,22 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
             _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-I{HOST / 'include'}", f"-I{INCLUDE}",
                   "-I/usr/local/cuda/include", *map(str, hsrcs), "-o", str(HOST_LIB),
                   f"-L{PKG}", "-lp3dcuda", "-Wl,-rpath,$ORIGIN"], verbose)
+    _build_bind(force, verbose)
     return LIB
+
+
+def _build_bind(force: bool, verbose: bool) -> None:
+    """_bind.so: rebuilt when its source, the C header or torch itself changes."""
+    import importlib.util
+    import sysconfig
+    torch = Path(importlib.util.find_spec("torch").origin).parent
+    if not force and not _stale(BIND_LIB, BIND, [INCLUDE / "p3d.h", torch / "version.py"]):
+        return
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-I{INCLUDE}", f"-isystem{torch / 'include'}",
+          f"-isystem{torch / 'include' / 'torch' / 'csrc' / 'api' / 'include'}", "-I/usr/local/cuda/include",
+          f"-I{sysconfig.get_paths()['include']}", str(BIND), "-o", str(BIND_LIB), f"-L{PKG}", "-lp3dcuda",
+          f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10",
+          "-Wl,-rpath,$ORIGIN"], verbose)
 
 
 def main() -> None:

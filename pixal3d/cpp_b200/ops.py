@@ -10,12 +10,15 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-import threading
 
 import torch
 
 from . import _lib as L
 from ._lib import P3DError
+try:
+    from . import _bind
+except ImportError as e:
+    raise ImportError("pixal3d/cpp_b200/_bind.so is not built for this torch; run `python -m pixal3d.cpp_b200.build`") from e
 
 _CTX: dict[int, "Context"] = {}
 
@@ -30,20 +33,11 @@ class Context:
             raise P3DError(rc, f"p3d_ctx_create(device={device}) failed")
         self.h = h
         self.device = device
-        self.lock = threading.Lock()
 
     def bind(self) -> "Context":
         s = torch.cuda.current_stream(self.device).cuda_stream
         L.lib.p3d_ctx_set_stream(self.h, C.c_void_p(s))
         return self
-
-    def call(self, fn, *args) -> None:
-        """fn(ctx, *args) on torch's current stream, checked.  Threads that
-        share the context take turns, so that none launches on the stream
-        another has just bound."""
-        with self.lock:
-            L.lib.p3d_ctx_set_stream(self.h, torch._C._cuda_getCurrentRawStream(self.device))
-            self.check(fn(self.h, *args))
 
     def check(self, rc: int) -> None:
         if rc != 0:
@@ -69,40 +63,16 @@ def ctx(device: torch.device | int | None = None) -> Context:
     return _CTX[idx].bind()
 
 
-def _ctx_on(what: str, t: torch.Tensor) -> Context:
-    """The context of t's device."""
-    idx = t.get_device()
-    c = _CTX.get(idx)
-    if c is None:
-        if idx < 0:
-            raise ValueError(f"{what}: tensors must be on a CUDA device")
-        c = _CTX.setdefault(idx, Context(idx))
-    return c
+def _context_handle(device: int) -> int:
+    return ctx(device).h.value
+
+
+_bind.setup(_context_handle, P3DError)
 
 
 def _need(ok: bool, message: str) -> None:
     if not ok:
         raise ValueError(message)
-
-
-def _matrix(what: str, t: torch.Tensor, cols: int, dtype: torch.dtype, device: int) -> int:
-    """Row pitch (elements) of a 2-D view of `cols` columns with unit column
-    stride; of a single row, `cols` (its stride says nothing)."""
-    if t.ndim != 2 or t.dtype is not dtype or t.get_device() != device or t.shape[1] != cols:
-        raise ValueError(f"{what}: expected a 2-D {dtype} tensor of {cols} columns on cuda:{device}")
-    pitch, unit = t.stride()
-    if unit != 1 and cols > 1:
-        raise ValueError(f"{what}: expected a row-major view")
-    return pitch if t.shape[0] > 1 else cols
-
-
-def _vector(what: str, t: torch.Tensor | None, n: int, dtype: torch.dtype, device: int):
-    """Pointer of a contiguous 1-D tensor of n elements, or None."""
-    if t is None:
-        return None
-    if t.dtype is not dtype or t.shape != (n,) or t.get_device() != device or not t.is_contiguous():
-        raise ValueError(f"{what}: expected a contiguous {dtype} vector of {n} on cuda:{device}")
-    return t.data_ptr()
 
 
 def _p(t: torch.Tensor | None):
@@ -119,7 +89,6 @@ def _dt(t: torch.Tensor) -> int:
     raise TypeError(f"unsupported dtype {t.dtype}")
 
 
-_DTYPES = {torch.float32: L.P3D_F32, torch.bfloat16: L.P3D_BF16, torch.float16: L.P3D_F16}
 HALF = (torch.bfloat16, torch.float16)
 
 
@@ -277,25 +246,7 @@ def quantize_rows(x: torch.Tensor, out: torch.Tensor | None = None,
     scale = max|row| / 127, q = x / scale to the nearest, ties to even.  x
     [m, k] f32, bf16 or f16, any row pitch.  Returns (q [m, k] int8, scale
     [m]); a new q has rows of whole 16-byte words, as linear_i8 takes them."""
-    c = _ctx_on("quantize_rows", x)
-    dev, dt = c.device, _DTYPES.get(x.dtype)
-    if dt is None:
-        raise TypeError(f"quantize_rows: unsupported dtype {x.dtype}")
-    m, k = x.shape
-    _need(k > 0, "quantize_rows: rows of no elements")
-    ldx = _matrix("quantize_rows", x, k, x.dtype, dev)
-    if out is None:
-        ldq = (k + 15) & ~15
-        out = torch.empty_strided((m, k), (ldq, 1), dtype=torch.int8, device=x.device)
-    else:
-        ldq = _matrix("quantize_rows: out", out, k, torch.int8, dev)
-        _need(out.shape[0] == m, "quantize_rows: out must be of x's shape")
-    if scale is None:
-        scale = torch.empty(m, dtype=torch.float32, device=x.device)
-    ps = _vector("quantize_rows: scale", scale, m, torch.float32, dev)
-    if m:
-        c.call(L.lib.p3d_quantize_rows, x.data_ptr(), ldx, m, k, dt, out.data_ptr(), ldq, ps)
-    return out, scale
+    return _bind.quantize_rows(x, out, scale)
 
 
 def linear_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
@@ -305,41 +256,7 @@ def linear_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     """epilogue((x W^T) x_scale[row] w_scale[col] + b) on 8-bit integers
     (p3d_linear_i8): x [m, k] and w [n, k] int8 as quantize_rows makes them,
     scales and bias f32.  gate [items, n] f32 and batch_offsets as in linear."""
-    c = _ctx_on("linear_i8", x)
-    dev = c.device
-    m, k = x.shape
-    n = w.shape[0]
-    _need(k > 0 and n > 0, "linear_i8: x or w of no elements")
-    ldx, ldw = _matrix("linear_i8: x", x, k, torch.int8, dev), _matrix("linear_i8: w", w, k, torch.int8, dev)
-    if m == 1 or n == 1:  # a lone row has no pitch; the tensor maps want one of whole 16-byte words
-        ldx, ldw = (k + 15) & ~15 if m == 1 else ldx, (k + 15) & ~15 if n == 1 else ldw
-    if out is None:
-        _need(not epilogue & L.EPI_RESIDUAL, "linear_i8: the residual epilogue adds into out")
-        out = torch.empty(m, n, dtype=out_dtype, device=x.device)
-        ldo = n
-    else:
-        out_dtype = out.dtype
-        ldo = _matrix("linear_i8: out", out, n, out_dtype, dev)
-        _need(out.shape[0] == m, "linear_i8: out must be [m, n]")
-    dt = _DTYPES.get(out_dtype)
-    if dt is None:
-        raise TypeError(f"linear_i8: unsupported output dtype {out_dtype}")
-    pxs, pws = (_vector("linear_i8: x_scale", x_scale, m, torch.float32, dev),
-                _vector("linear_i8: w_scale", w_scale, n, torch.float32, dev))
-    pb = _vector("linear_i8: bias", bias, n, torch.float32, dev)
-    pg = po = None
-    nb = gate_ld = 0
-    if gate is not None:
-        _need(batch_offsets is not None and batch_offsets.shape[0] > 1, "linear_i8: gate needs batch offsets")
-        nb = batch_offsets.shape[0] - 1
-        po = _vector("linear_i8: batch_offsets", batch_offsets, nb + 1, torch.int32, dev)
-        gate_ld = _matrix("linear_i8: gate", gate, n, torch.float32, dev)
-        _need(gate.shape[0] == nb, "linear_i8: gate must be [items, n]")
-        pg = gate.data_ptr()
-    if m:
-        c.call(L.lib.p3d_linear_i8, x.data_ptr(), ldx, pxs, w.data_ptr(), ldw, pws, pb, m, n, k, out.data_ptr(), ldo, dt,
-               epilogue, pg, gate_ld, po, nb)
-    return out
+    return _bind.linear_i8(x, x_scale, w, w_scale, bias, out, out_dtype, epilogue, gate, batch_offsets)
 
 
 def subm_conv3d(x: torch.Tensor, nbr: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None,
@@ -417,40 +334,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     doc_k equals doc_q; scores are softcap * tanh(score / softcap) -
     slopes[head] * |position - j|.  A query that sees nothing gets zeros; rows
     of a new out behind the last sequence are not written."""
-    c = _ctx_on("masked_attention", q)
-    dev, t, dt = c.device, q.dtype, _DTYPES.get(q.dtype)
-    _need(t is torch.bfloat16 or t is torch.float16, "masked_attention: q, k, v must be bf16 or f16")
-    if kv_heads is None:
-        kv_heads = heads
-    rows_q, width = q.shape
-    rows_k = k.shape[0]
-    _need(heads > 0 and kv_heads > 0 and width % heads == 0, "masked_attention: q's columns must be heads * d")
-    d = width // heads
-    ldq = _matrix("masked_attention: q", q, width, t, dev)
-    ldk, ldv = _matrix("masked_attention: k", k, kv_heads * d, t, dev), _matrix("masked_attention: v", v, kv_heads * d, t, dev)
-    _need(v.shape[0] == rows_k, "masked_attention: k and v must have the same rows")
-    nseq = cu_q.shape[0] - 1
-    pcq, pck = (_vector("masked_attention: cu_q", cu_q, nseq + 1, torch.int32, dev),
-                _vector("masked_attention: cu_k", cu_k, nseq + 1, torch.int32, dev))
-    if out is None:
-        out = torch.empty(rows_q, width, dtype=t, device=q.device)
-        ldo = width
-    else:
-        ldo = _matrix("masked_attention: out", out, width, t, dev)
-        _need(out.shape[0] == rows_q, "masked_attention: out must be like q")
-    _need((doc_q is None) == (doc_k is None), "masked_attention: doc_q and doc_k go together")
-    rules = L.AttentionRules(softcap, causal, _vector("masked_attention: prefix", prefix, nseq, torch.int32, dev),
-                             _vector("masked_attention: doc_q", doc_q, rows_q, torch.int32, dev),
-                             _vector("masked_attention: doc_k", doc_k, rows_k, torch.int32, dev),
-                             _vector("masked_attention: slopes", slopes, heads, torch.float32, dev))
-    max_q, max_k = min(max_q, rows_q), min(max_k, rows_k)
-    if rows_q == 0 or nseq <= 0 or max_q <= 0:
-        return out
-    wsb = L.lib.p3d_masked_attention_workspace(nseq, max_q, max_k, rows_q, rows_k, heads, kv_heads, d, doc_k is not None)
-    ws = torch.empty(wsb, dtype=torch.uint8, device=q.device) if wsb else None
-    c.call(L.lib.p3d_masked_attention, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo, pcq, pck,
-           nseq, max_q, max_k, rows_q, rows_k, heads, kv_heads, d, scale, C.byref(rules), ws.data_ptr() if wsb else None, wsb, dt)
-    return out
+    return _bind.masked_attention(q, k, v, cu_q, cu_k, max_q, max_k, heads, scale, kv_heads, causal, prefix, doc_q, doc_k, slopes,
+                                  softcap, out)
 
 
 def window_partition(coords: torch.Tensor, batch: int, window: int, shift: int, spatial) -> tuple:
@@ -627,28 +512,10 @@ def rotary(x: torch.Tensor, freqs: torch.Tensor, heads: int, head_dim: int, posi
     rot/2) ("half") or (2i, 2i + 1) ("interleaved") with rot = 2 * len(freqs);
     the head's other elements are copied.  positions int32, None for
     position_offset + row.  out may be x itself."""
-    c = _ctx_on("rotary", x)
-    dev, t = c.device, x.dtype
-    dt, lay = _DTYPES.get(t), ROTARY_LAYOUTS.get(layout)
-    if dt is None:
-        raise TypeError(f"rotary: unsupported dtype {t}")
-    _need(lay is not None, "rotary: layout must be half or interleaved")
-    n, width = x.shape
-    _need(width == heads * head_dim, "rotary: x must be [n, heads * head_dim]")
-    ldx = _matrix("rotary", x, width, t, dev)
-    if out is None:
-        out = torch.empty(n, width, dtype=t, device=x.device)
-        ldo = width
-    else:
-        ldo = _matrix("rotary: out", out, width, t, dev)
-        _need(out.shape[0] == n, "rotary: out must be like x")
-    half = freqs.shape[0]
-    pf = _vector("rotary: freqs", freqs, half, torch.float64, dev)
-    pp = _vector("rotary: positions", positions, n, torch.int32, dev)
-    if n:
-        c.call(L.lib.p3d_rotary, x.data_ptr(), ldx, n, heads, head_dim, 2 * half, lay, pp, position_offset, pf, amplitude,
-               out.data_ptr(), ldo, dt)
-    return out
+    lay = ROTARY_LAYOUTS.get(layout)
+    if lay is None:
+        raise ValueError("rotary: layout must be half or interleaved")
+    return _bind.rotary(x, freqs, heads, head_dim, positions, lay, amplitude, position_offset, out)
 
 
 def activation(x: torch.Tensor, act: int) -> torch.Tensor:
