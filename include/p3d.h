@@ -248,7 +248,7 @@ int p3d_linear_headnorm(p3d_ctx *ctx, const void *x, int64_t ldx, const void *w,
  * or a NaN gets the scale NaN and zeros, so products with it are NaN.  x
  * [m][ldx] of dtype, q [m][ldq], scale f32 [m]; columns [0, k) of q are
  * written.  Any k and any leading dimensions >= k; rows on 16-byte boundaries
- * are read fastest.  Quantises activations by token and weights [n][k] by
+ * are written fastest.  Quantises activations by token and weights [n][k] by
  * output channel. */
 int p3d_quantize_rows(p3d_ctx *ctx, const void *x, int64_t ldx, int64_t m, int64_t k, int dtype, int8_t *q,
                       int64_t ldq, float *scale);

@@ -46,6 +46,20 @@ def test_quantize_rows_exact(dtype, m, k):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("k", [8, 31, 129, 256, 257, 1000, 1024, 1031, 2048, 2060, 4099, 8192, 16400])
+def test_quantize_rows_every_width(dtype, k):
+    """Rows enough for the per-row thread counts of large calls, rows that
+    start inside a 16-byte word among them."""
+    g = torch.Generator(device="cuda").manual_seed(k)
+    x = torch.randn((301, k), device="cuda", generator=g).to(dtype)
+    check_quantised(x)
+    wide = torch.randn((301, k + 3), device="cuda", generator=g).to(dtype)
+    wide[:, 0] = math.nan  # beside the rows, in the words they begin in
+    wide[:, k + 1:] = math.inf
+    check_quantised(wide[:, 1:k + 1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("pad,off", [(1, 0), (3, 1), (8, 8), (27, 0), (16, 3)])
 def test_quantize_rows_strided(dtype, pad, off):
     """Rows inside wider ones, at any alignment; q beside its columns stays as it was."""
