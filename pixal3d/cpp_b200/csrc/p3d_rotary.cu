@@ -8,7 +8,14 @@
 // turns off, 2e-7 rad, whatever the position), then sincospif.
 //
 // Bound by HBM: the rows are read and written once, and the rot/2 angles of a
-// token are computed once for all of its heads, into shared memory.
+// token are computed once for all of its heads in a block, into shared memory,
+// while the block's first rows are on their way.
+//
+// Where rows lie on 16-byte boundaries and no pair crosses its vectors (half:
+// dim and rot/2 whole vectors; interleaved: dim even), a thread turns vectors
+// in registers, four of them in flight.  Everything else goes through shared
+// memory: the block's heads are copied there as they lie, turned there and
+// copied out.
 #include <algorithm>
 
 #include "p3d_common.cuh"
@@ -18,6 +25,13 @@ namespace {
 
 constexpr int kRotThreads = 256;
 constexpr int kMaxRotDim = 512;
+
+// n / d and n % d for n d < 2^32, d > 1 (a rounded-up reciprocal).
+struct Divisor {
+    uint32_t d, r;
+    explicit Divisor(uint32_t v = 1) : d(v), r(v > 1 ? static_cast<uint32_t>(((uint64_t(1) << 32) + v - 1) / v) : 0) {}
+    __device__ __forceinline__ uint32_t div(uint32_t n) const { return d > 1 ? __umulhi(n, r) : n; }
+};
 
 struct RotaryParams {
     const void *x;
@@ -30,131 +44,217 @@ struct RotaryParams {
     const double *freqs;  // [half]
     float amplitude;
     int heads, dim, half;
-    int tokens;  // per block
+    int tokens, group;  // tokens and heads of a block
+    int items;          // vectors (items) of one token's heads in a block
+    Divisor per_token, per_head, by_half;
+    int vectors;  // staged kernel: rows and heads' groups lie on 16-byte boundaries
 };
 
-template <typename T, int VEC>
-struct Vec {
-    float v[VEC];
-    __device__ __forceinline__ void load(const T *p) {
-        if constexpr (VEC * sizeof(T) == 16) {
-            const uint4 u = *reinterpret_cast<const uint4 *>(p);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (sizeof(T) == 4) {
-                    v[i] = __uint_as_float(w[i]);
-                } else {
-                    const float2 f = unpack2<T>(w[i]);
-                    v[2 * i] = f.x;
-                    v[2 * i + 1] = f.y;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) v[i] = to_f32(p[i]);
-        }
-    }
-    __device__ __forceinline__ void store(T *p) const {
-        if constexpr (VEC * sizeof(T) == 16) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (sizeof(T) == 4)
-                    w[i] = __float_as_uint(v[i]);
-                else
-                    w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
-            }
-            *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) p[i] = from_f32<T>(v[i]);
-        }
-    }
-};
-
-// An item is VEC pairs of one head: two vectors half apart (half layout) or
-// 2 VEC consecutive elements (interleaved); then the copied elements, 2 VEC an
-// item.  Every item reads all of its elements before it writes them, so out
-// may be x itself.
-template <typename T, int VEC, bool HALF>
-__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryParams p) {
-    extern __shared__ float2 table[];  // [tokens][half] (cos, sin) times the amplitude
-    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tokens;
-    const int nt = static_cast<int>(min(static_cast<int64_t>(p.tokens), p.n - t0));
-    for (int e = threadIdx.x; e < nt * p.half; e += kRotThreads) {
-        const int64_t row = t0 + e / p.half;
+// Cosines and sines, times the amplitude, of the block's tokens: [tokens][half].
+__device__ __forceinline__ void rotary_table(const RotaryParams &p, float2 *table, int64_t t0, int nt) {
+    for (uint32_t e = threadIdx.x; e < static_cast<uint32_t>(nt * p.half); e += kRotThreads) {
+        const uint32_t tok = p.by_half.div(e), i = e - tok * p.half;
+        const int64_t row = t0 + tok;
         const double pos = static_cast<double>(p.positions ? p.positions[row] : p.offset + row);
-        const double turns = pos * (__ldg(p.freqs + e % p.half) * 0.15915494309189533577);
+        const double turns = pos * (__ldg(p.freqs + i) * 0.15915494309189533577);
         float s, c;
         sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
         table[e] = make_float2(p.amplitude * c, p.amplitude * s);
     }
-    __syncthreads();
-    const int turned = p.half / VEC;                                    // items of turned pairs per head
-    const int rest = p.dim - 2 * p.half;                                // copied elements per head
-    const int iph = turned + (rest + 2 * VEC - 1) / (2 * VEC);          // items per head
-    const int ipt = iph * p.heads;                                      // per token
-    for (int e = threadIdx.x; e < nt * ipt; e += kRotThreads) {
-        const int tok = e / ipt, in = e % ipt, head = in / iph, i = in % iph;
-        const T *xr = static_cast<const T *>(p.x) + (t0 + tok) * p.ldx + static_cast<int64_t>(head) * p.dim;
-        T *yr = static_cast<T *>(p.out) + (t0 + tok) * p.ldo + static_cast<int64_t>(head) * p.dim;
-        if (i < turned) {
-            const float2 *cs = table + tok * p.half + i * VEC;
-            const int ia = HALF ? i * VEC : 2 * i * VEC, ib = HALF ? ia + p.half : ia + VEC;
-            Vec<T, VEC> a, b;
-            a.load(xr + ia);
-            b.load(xr + ib);
-            if constexpr (HALF) {
+}
+
+// 16 bytes as elements.
+template <typename T>
+struct Vec {
+    static constexpr int N = 16 / sizeof(T);
+    float v[N];
+    __device__ __forceinline__ explicit Vec(const uint4 &u) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const float u = a.v[j], w = b.v[j];
-                    a.v[j] = u * cs[j].x - w * cs[j].y;
-                    b.v[j] = u * cs[j].y + w * cs[j].x;
-                }
-            } else if constexpr (VEC == 1) {
-                const float u = a.v[0], w = b.v[0];
-                a.v[0] = u * cs[0].x - w * cs[0].y;
-                b.v[0] = u * cs[0].y + w * cs[0].x;
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                v[i] = __uint_as_float(w[i]);
             } else {
-#pragma unroll
-                for (int j = 0; j < VEC / 2; ++j) {
-                    const float u = a.v[2 * j], w = a.v[2 * j + 1];
-                    a.v[2 * j] = u * cs[j].x - w * cs[j].y;
-                    a.v[2 * j + 1] = u * cs[j].y + w * cs[j].x;
-                    const float u2 = b.v[2 * j], w2 = b.v[2 * j + 1];
-                    b.v[2 * j] = u2 * cs[VEC / 2 + j].x - w2 * cs[VEC / 2 + j].y;
-                    b.v[2 * j + 1] = u2 * cs[VEC / 2 + j].y + w2 * cs[VEC / 2 + j].x;
-                }
+                const float2 f = unpack2<T>(w[i]);
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
             }
-            a.store(yr + ia);
-            b.store(yr + ib);
-        } else {
-            const int c0 = 2 * p.half + (i - turned) * 2 * VEC;
+        }
+    }
+    __device__ __forceinline__ uint4 bits() const {
+        uint32_t w[4];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int c = c0 + j * VEC;
-                if (c >= p.dim) break;
-                Vec<T, VEC> a;
-                a.load(xr + c);
-                a.store(yr + c);
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4)
+                w[i] = __float_as_uint(v[i]);
+            else
+                w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
+__device__ __forceinline__ void turn(float &a, float &b, const float2 &cs) {
+    const float u = a, w = b;
+    a = u * cs.x - w * cs.y;
+    b = u * cs.y + w * cs.x;
+}
+
+// Half: an item is the vectors i and i + half of a head, then the copied
+// vectors one by one.  Interleaved: an item is one vector of a head.  Every
+// item is read before it is written and no other reads it, so out may be x.
+template <typename T, bool HALF>
+__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryParams p) {
+    constexpr int N = Vec<T>::N;
+    constexpr int FLY = HALF ? 2 : 4;  // items in flight
+    extern __shared__ float2 table[];
+    pdl_wait();
+    pdl_trigger();
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tokens;
+    const int nt = static_cast<int>(min(static_cast<int64_t>(p.tokens), p.n - t0));
+    const int pairs = p.half / N;  // half: items that turn, of a head
+    const uint32_t total = static_cast<uint32_t>(nt * p.items);
+    for (uint32_t e0 = threadIdx.x; e0 - threadIdx.x < total; e0 += FLY * kRotThreads) {
+        uint4 a[FLY], b[HALF ? FLY : 1];
+        int64_t at[FLY];
+        int tok[FLY], i[FLY];
+#pragma unroll
+        for (int f = 0; f < FLY; ++f) {
+            const uint32_t e = e0 + f * kRotThreads;
+            tok[f] = p.tokens > 1 ? p.per_token.div(e) : 0;
+            const uint32_t in = e - tok[f] * p.items, head = p.per_head.div(in);
+            i[f] = in - head * p.per_head.d;
+            const int elem = HALF ? (i[f] < pairs ? i[f] : i[f] + pairs) * N : i[f] * N;
+            at[f] = static_cast<int64_t>(head) * p.dim + elem;
+            if (e < total) {
+                const T *x = static_cast<const T *>(p.x) + (t0 + tok[f]) * p.ldx + at[f];
+                a[f] = *reinterpret_cast<const uint4 *>(x);
+                if (HALF && i[f] < pairs) b[HALF ? f : 0] = *reinterpret_cast<const uint4 *>(x + p.half);
+            }
+        }
+        if (e0 == threadIdx.x) {
+            rotary_table(p, table, t0, nt);
+            __syncthreads();
+        }
+#pragma unroll
+        for (int f = 0; f < FLY; ++f) {
+            if (e0 + f * kRotThreads >= total) break;
+            T *y = static_cast<T *>(p.out) + (t0 + tok[f]) * p.ldo + at[f];
+            const float2 *cs = table + tok[f] * p.half;
+            if constexpr (HALF) {
+                if (i[f] < pairs) {
+                    Vec<T> u(a[f]), w(b[f]);
+#pragma unroll
+                    for (int j = 0; j < N; ++j) turn(u.v[j], w.v[j], cs[i[f] * N + j]);
+                    *reinterpret_cast<uint4 *>(y) = u.bits();
+                    *reinterpret_cast<uint4 *>(y + p.half) = w.bits();
+                } else {
+                    *reinterpret_cast<uint4 *>(y) = a[f];
+                }
+            } else {
+                Vec<T> u(a[f]);
+                const int first = i[f] * (N / 2);  // pair
+#pragma unroll
+                for (int j = 0; j < N / 2; ++j)
+                    if (first + j < p.half) turn(u.v[2 * j], u.v[2 * j + 1], cs[first + j]);
+                *reinterpret_cast<uint4 *>(y) = u.bits();
             }
         }
     }
 }
 
-template <typename T, int VEC>
-int launch_rotary(p3d_ctx *ctx, RotaryParams p, int layout) {
-    // about 1024 items a block, so the angles are spread over few tokens
-    const int ipt = p.heads * ((p.dim / 2 + VEC - 1) / VEC);
-    p.tokens = std::max(1, std::min({1024 / std::max(ipt, 1), 4096 / p.half, 64}));
-    const size_t smem = sizeof(float2) * p.tokens * p.half;
-    const unsigned grid = static_cast<unsigned>(ceil_div(p.n, p.tokens));
-    if (layout == P3D_ROTARY_HALF)
-        rotary_kernel<T, VEC, true><<<grid, kRotThreads, smem, ctx->stream>>>(p);
-    else
-        rotary_kernel<T, VEC, false><<<grid, kRotThreads, smem, ctx->stream>>>(p);
-    return check_launch(ctx, "rotary");
+// Any layout: `group` heads of `tokens` tokens through shared memory.
+template <typename T, bool HALF>
+__global__ void __launch_bounds__(kRotThreads) rotary_staged_kernel(const RotaryParams p) {
+    constexpr int N = Vec<T>::N;
+    extern __shared__ float2 table[];
+    T *rows = reinterpret_cast<T *>(table + ((p.tokens * p.half + 1) & ~1));  // [tokens][group * dim], 16-byte aligned
+    pdl_wait();
+    pdl_trigger();
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tokens;
+    const int nt = static_cast<int>(min(static_cast<int64_t>(p.tokens), p.n - t0));
+    const int head0 = blockIdx.y * p.group;
+    const int wide = p.group * p.dim;                            // staged elements of a token
+    const int width = min(p.group, p.heads - head0) * p.dim;     // of them present
+    const int64_t col = static_cast<int64_t>(head0) * p.dim;
+    if (p.vectors) {
+        for (int tok = 0; tok < nt; ++tok) {
+            const T *x = static_cast<const T *>(p.x) + (t0 + tok) * p.ldx + col;
+            for (int c = threadIdx.x * N; c < width; c += kRotThreads * N) cp_async16(rows + tok * wide + c, x + c, 16);
+        }
+        cp_async_commit();
+    } else {
+        for (int tok = 0; tok < nt; ++tok) {
+            const T *x = static_cast<const T *>(p.x) + (t0 + tok) * p.ldx + col;
+#pragma unroll 4
+            for (int c = threadIdx.x; c < width; c += kRotThreads) rows[tok * wide + c] = x[c];
+        }
+    }
+    rotary_table(p, table, t0, nt);
+    cp_async_wait<0>();
+    __syncthreads();
+    // the pairs are turned where they lie
+    const uint32_t pairs = static_cast<uint32_t>(width / p.dim * p.half);
+    for (int tok = 0; tok < nt; ++tok) {
+        T *from = rows + tok * wide;
+        const float2 *cs = table + tok * p.half;
+#pragma unroll 4
+        for (uint32_t e = threadIdx.x; e < pairs; e += kRotThreads) {
+            const uint32_t head = p.by_half.div(e), i = e - head * p.half;
+            T *h = from + head * p.dim;
+            T &a = HALF ? h[i] : h[2 * i], &b = HALF ? h[i + p.half] : h[2 * i + 1];
+            float u = to_f32(a), w = to_f32(b);
+            turn(u, w, cs[i]);
+            a = from_f32<T>(u);
+            b = from_f32<T>(w);
+        }
+    }
+    __syncthreads();
+    for (int tok = 0; tok < nt; ++tok) {
+        T *y = static_cast<T *>(p.out) + (t0 + tok) * p.ldo + col;
+        const T *from = rows + tok * wide;
+        if (p.vectors) {
+            for (int c = threadIdx.x * N; c < width; c += kRotThreads * N)
+                *reinterpret_cast<uint4 *>(y + c) = *reinterpret_cast<const uint4 *>(from + c);
+        } else {
+#pragma unroll 4
+            for (int c = threadIdx.x; c < width; c += kRotThreads) y[c] = from[c];
+        }
+    }
+}
+
+template <typename T, bool HALF>
+int launch_rotary(p3d_ctx *ctx, RotaryParams p) {
+    constexpr int N = Vec<T>::N, es = sizeof(T);
+    const uintptr_t xa = reinterpret_cast<uintptr_t>(p.x), oa = reinterpret_cast<uintptr_t>(p.out);
+    const bool rows16 = (xa | oa) % 16 == 0 && (p.n == 1 || (p.ldx % N == 0 && p.ldo % N == 0));
+    p.by_half = Divisor(p.half);
+    const int iph = HALF ? (p.dim - p.half) / N : p.dim / N;  // items of a head
+    if (rows16 && p.dim % N == 0 && (!HALF || p.half % N == 0) && static_cast<int64_t>(p.heads) * iph < (1 << 24)) {
+        p.per_head = Divisor(iph);
+        p.items = p.heads * iph;
+        // 1024 items a block, so the angles are spread over few tokens, and a
+        // few tokens' rows keep every thread's vectors in flight
+        p.tokens = std::max(1, std::min({1024 / p.items, 4096 / p.half, 64}));
+        p.per_token = Divisor(p.items);
+        P3D_CUDA(ctx, launch_pdl(rotary_kernel<T, HALF>, dim3(static_cast<unsigned>(ceil_div(p.n, p.tokens))), dim3(kRotThreads),
+                                 sizeof(float2) * p.tokens * p.half, ctx->stream, p));
+        return check_launch(ctx, "rotary");
+    }
+    // whole groups of N heads start on 16-byte boundaries of aligned rows, whatever dim is
+    p.group = std::min(p.heads, std::max(N, 16384 / es / p.dim / N * N));
+    p.vectors = rows16 && static_cast<int64_t>(p.heads) * p.dim % N == 0;
+    p.tokens = std::max(1, std::min({16384 / (p.group * p.dim * es), 1024 / p.half, 16}));
+    const size_t smem = sizeof(float2) * ((p.tokens * p.half + 1) & ~1) + static_cast<size_t>(p.tokens) * p.group * p.dim * es;
+    P3D_CUDA(ctx, launch_pdl(rotary_staged_kernel<T, HALF>,
+                             dim3(static_cast<unsigned>(ceil_div(p.n, p.tokens)), static_cast<unsigned>(ceil_div(p.heads, p.group))),
+                             dim3(kRotThreads), smem, ctx->stream, p));
+    return check_launch(ctx, "rotary_staged");
+}
+
+template <typename T>
+int launch_layout(p3d_ctx *ctx, const RotaryParams &p, int layout) {
+    return layout == P3D_ROTARY_HALF ? launch_rotary<T, true>(ctx, p) : launch_rotary<T, false>(ctx, p);
 }
 
 }  // namespace
@@ -187,15 +287,21 @@ extern "C" int p3d_rotary(p3d_ctx *ctx, const void *x, int64_t ldx, int64_t n, i
                          (xa > oa ? xa - oa : oa - xa) % (ldx * es) >= width * es &&
                          (xa > oa ? xa - oa : oa - xa) % (ldx * es) <= (ldx - width) * es),
                 "p3d_rotary: out must be x itself or not overlap it");
-    RotaryParams p{x, ldx, out, ldo, n, positions, position_offset, freqs, amplitude, heads, head_dim, rot_dim / 2, 1};
+    RotaryParams p{};
+    p.x = x;
+    p.ldx = ldx;
+    p.out = out;
+    p.ldo = ldo;
+    p.n = n;
+    p.positions = positions;
+    p.offset = position_offset;
+    p.freqs = freqs;
+    p.amplitude = amplitude;
+    p.heads = heads;
+    p.dim = head_dim;
+    p.half = rot_dim / 2;
     DeviceGuard on(ctx->device);
-    // 16-byte vectors where rows, heads and both elements of the pairs allow
-    // them, single elements elsewhere
-    const int vec = static_cast<int>(16 / es);
-    const bool aligned = (xa | oa) % 16 == 0 && (n == 1 || (ldx % vec == 0 && ldo % vec == 0)) && head_dim % vec == 0 &&
-                         p.half % vec == 0;
-    if (dtype == P3D_F32) return aligned ? launch_rotary<float, 4>(ctx, p, layout) : launch_rotary<float, 1>(ctx, p, layout);
-    if (dtype == P3D_BF16)
-        return aligned ? launch_rotary<__nv_bfloat16, 8>(ctx, p, layout) : launch_rotary<__nv_bfloat16, 1>(ctx, p, layout);
-    return aligned ? launch_rotary<__half, 8>(ctx, p, layout) : launch_rotary<__half, 1>(ctx, p, layout);
+    if (dtype == P3D_F32) return launch_layout<float>(ctx, p, layout);
+    if (dtype == P3D_BF16) return launch_layout<__nv_bfloat16>(ctx, p, layout);
+    return launch_layout<__half>(ctx, p, layout);
 }
