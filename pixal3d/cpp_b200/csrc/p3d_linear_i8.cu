@@ -81,12 +81,14 @@ __device__ __forceinline__ void store_one(const I8Params &p, int64_t row, int64_
         static_cast<__half *>(p.out)[row * p.ldo + col] = __float2half_rn(v);
 }
 
-// 16 bytes of a row from byte k on; bytes at or past K are zero (and not read).
-__device__ __forceinline__ int4 load16(const int8_t *row, int k, int K) {
-    if (k + 16 <= K) return __ldg(reinterpret_cast<const int4 *>(row + k));
-    uint32_t w[4] = {0, 0, 0, 0};
-    for (int i = 0; i < 16 && k + i < K; ++i) w[i / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(row[k + i])) << (8 * (i % 4));
-    return make_int4(w[0], w[1], w[2], w[3]);
+// 16 bytes of a row from byte k on.  The word that holds the row's end is read
+// whole (rows start on 16-byte boundaries, so it lies in the same allocation).
+__device__ __forceinline__ int4 load16(const int8_t *row, int k) { return __ldg(reinterpret_cast<const int4 *>(row + k)); }
+// Bytes at or past K to zero; one operand is enough.
+__device__ __forceinline__ int4 trim16(const int4 &v, int k, int K) {
+    auto keep = [&](int w, int n) { return n >= 4 ? w : n <= 0 ? 0 : static_cast<int>(static_cast<uint32_t>(w) & ((1u << (8 * n)) - 1u)); };
+    const int n = K - k;
+    return n >= 16 ? v : make_int4(keep(v.x, n), keep(v.y, n - 4), keep(v.z, n - 8), keep(v.w, n - 12));
 }
 
 // Few rows: a warp takes NC channels and MR rows, its lanes stride over k.
@@ -116,10 +118,10 @@ __global__ void __launch_bounds__(kRowThreads) linear_i8_rows_kernel(const I8Par
     for (int k = lane * 16; k < p.K; k += 512) {
         int4 b[NC];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) b[c] = load16(wr[c], k, p.K);
+        for (int c = 0; c < NC; ++c) b[c] = trim16(load16(wr[c], k), k, p.K);
 #pragma unroll
         for (int r = 0; r < MR; ++r) {
-            const int4 a = load16(xr[r], k, p.K);
+            const int4 a = load16(xr[r], k);
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 acc[r][c] = __dp4a(a.x, b[c].x, acc[r][c]);
@@ -265,13 +267,14 @@ __device__ __forceinline__ void finish32(const I8Params &p, float (&v)[32], floa
     }
 }
 
+__device__ __forceinline__ void prefetch_l1(const void *p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
+
 // One epilogue warp's columns of an accumulator: rows row0 .. row0 + 31 (lane
 // = row), columns n0 .. n0 + COLS - 1.
 template <int COLS>
 __device__ __forceinline__ void epilogue_i8(const I8Params &p, const CUtensorMap *tmo, uint32_t tacc, int64_t row0, int lane,
-                                            int64_t n0, uint8_t *buf) {
+                                            int64_t n0, float xs, uint8_t *buf) {
     const int64_t row = row0 + lane;
-    const float xs = row < p.M ? __ldg(p.xs + row) : 0.0f;
     const bool f32 = p.out_dtype == P3D_F32;
     // 64 bytes of each row (lane) to columns col..
     auto put = [&](const uint4 *w, int64_t col) {
@@ -463,11 +466,17 @@ __global__ void __launch_bounds__(kThreadsT, 1)
         uint32_t acc_phase = 0;
         for (int64_t t = first; t < tiles; t += step) {
             const int64_t m0 = t / n_tiles * kTileM + q * 32, n0 = t % n_tiles * BN + h * C::COLS;
+            // what the epilogue reads comes while the MMAs run
+            const float xs = m0 + lane < p.M ? __ldg(p.xs + m0 + lane) : 0.0f;
+            if (lane * 8 < C::COLS && n0 + lane * 8 < p.N) {
+                prefetch_l1(p.ws + n0 + lane * 8);
+                if (p.bias) prefetch_l1(p.bias + n0 + lane * 8);
+            }
             if (!warp_wait<false>(&tfull[acc], acc_phase, p.fault)) break;
             tc_fence_after();
             if (m0 < p.M)
                 epilogue_i8<C::COLS>(p, &tmap_o, tmem + acc * BN + h * C::COLS + (static_cast<uint32_t>(q * 32) << 16), m0,
-                                     lane, n0, buf);
+                                     lane, n0, xs, buf);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&tempty[acc]);

@@ -30,8 +30,10 @@
 namespace p3d {
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4;  // of a block that walks a range, and of the join
 constexpr int kThreadsR = 32 * kWarps;
+// A block that takes a whole item of few keys has 8 warps: half as many tiles
+// one after the other.
 
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -104,17 +106,17 @@ __device__ __forceinline__ int find_seq(const MaskedParams &p, int lane, int seq
     return p.nseq;
 }
 
-template <int D, int HT>
+template <int D, int HT, int W>
 struct RowsShared {
-    float o[kWarps][8 * HT][D + 4];  // + 4: the 8 dims a lane stores start in different banks for different heads
-    float m[kWarps][8 * HT], l[kWarps][8 * HT];
+    float o[W][8 * HT][D + 4];  // + 4: the 8 dims a lane stores start in different banks for different heads
+    float m[W][8 * HT], l[W][8 * HT];
 };
 
 // One item's key tiles [t0, t1): item `local` of sequence seq.  Writes the
 // output when `whole`, else the part `slot` (sums against its own maximum).
 // HT: 8 heads a block, or 16.
-template <typename T, int D, int HT>
-__device__ __forceinline__ void rows_item(const MaskedParams &p, RowsShared<D, HT> &sm, const SeqRange &sr, int seq, int local, int t0,
+template <typename T, int D, int HT, int W>
+__device__ __forceinline__ void rows_item(const MaskedParams &p, RowsShared<D, HT, W> &sm, const SeqRange &sr, int seq, int local, int t0,
                                           int t1, bool whole, int64_t slot) {
     constexpr int KC = D / 32;  // 16-byte chunks of a K row per lane
     constexpr int VS = D / 64;  // 64-dim slabs of V
@@ -186,9 +188,9 @@ __device__ __forceinline__ void rows_item(const MaskedParams &p, RowsShared<D, H
     };
     constexpr int kAhead = D == 64 ? 2 : 0;
     for (int a = 1; a < kAhead; ++a)
-        if (tile0 + warp + a * kWarps < tile1) prefetch(tile0 + warp + a * kWarps);
-    for (int tile = tile0 + warp; tile < tile1; tile += kWarps) {
-        if (kAhead > 0 && tile + kAhead * kWarps < tile1) prefetch(tile + kAhead * kWarps);
+        if (tile0 + warp + a * W < tile1) prefetch(tile0 + warp + a * W);
+    for (int tile = tile0 + warp; tile < tile1; tile += W) {
+        if (kAhead > 0 && tile + kAhead * W < tile1) prefetch(tile + kAhead * W);
         bool vis[4];
         uint4 vf[4][VS];
 #pragma unroll
@@ -213,7 +215,7 @@ __device__ __forceinline__ void rows_item(const MaskedParams &p, RowsShared<D, H
                     mma16816<T>(sc[t], a, word(kf[t][c], 2 * h), word(kf[t][c], 2 * h + 1));
                 }
         }
-        if (tile + kWarps < tile1) load_k(tile + kWarps);
+        if (tile + W < tile1) load_k(tile + W);
         float mx[HT];
         bool raised = false;
 #pragma unroll
@@ -297,16 +299,16 @@ __device__ __forceinline__ void rows_item(const MaskedParams &p, RowsShared<D, H
                         make_float4(o[s][2 * h][r][e], o[s][2 * h][r][2 + e], o[s][2 * h + 1][r][e], o[s][2 * h + 1][r][2 + e]);
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < nrows * (D / 4); e += kThreadsR) {
+    for (int e = threadIdx.x; e < nrows * (D / 4); e += 32 * W) {
         const int r = e / (D / 4), d = e % (D / 4) * 4;
         float mm = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sm.m[w][r]);
+        for (int w = 0; w < W; ++w) mm = fmaxf(mm, sm.m[w][r]);
         const float base = mm == -INFINITY ? 0.0f : mm;
         float ll = 0.0f;
         float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < W; ++w) {
             const float a = ex2f(sm.m[w][r] - base);
             const float4 x = *reinterpret_cast<const float4 *>(&sm.o[w][r][d]);
             ll = fmaf(sm.l[w][r], a, ll);
@@ -332,18 +334,27 @@ constexpr int rows_per_sm() {
     return (D == 64 ? 4 : 3) - (HT - 1);
 }
 
+template <int D, int HT>
+constexpr int item_warps() {
+    return D * HT > 128 ? 4 : 8;  // 16 heads of 128 would need 68 KB for the join
+}
 template <typename T, int D, int HT>
-__global__ void __launch_bounds__(kThreadsR, rows_per_sm<D, HT>()) masked_rows_kernel(const MaskedParams p) {
-    __shared__ RowsShared<D, HT> sm;
+__global__ void __launch_bounds__(32 * item_warps<D, HT>()) masked_items_kernel(const MaskedParams p) {
+    constexpr int W = item_warps<D, HT>();
+    __shared__ RowsShared<D, HT, W> sm;
+    pdl_wait();
+    pdl_trigger();
+    const SeqRange sr = seq_range(p, blockIdx.y);
+    if (static_cast<int>(blockIdx.x) < seq_items(p, sr))
+        rows_item<T, D, HT, W>(p, sm, sr, blockIdx.y, blockIdx.x, 0, item_tiles(sr), true, 0);
+}
+
+template <typename T, int D, int HT>
+__global__ void __launch_bounds__(kThreadsR, rows_per_sm<D, HT>()) masked_ranges_kernel(const MaskedParams p) {
+    __shared__ RowsShared<D, HT, kWarps> sm;
     pdl_wait();
     pdl_trigger();
     const int lane = threadIdx.x & 31;
-    if (p.ranges == 0) {  // a block an item
-        const SeqRange sr = seq_range(p, blockIdx.y);
-        if (static_cast<int>(blockIdx.x) < seq_items(p, sr))
-            rows_item<T, D, HT>(p, sm, sr, blockIdx.y, blockIdx.x, 0, item_tiles(sr), true, 0);
-        return;
-    }
     const int64_t total = all_tiles(p, lane);  // every warp finds the same
     int64_t x = total * blockIdx.x / p.ranges;
     const int64_t x1 = total * (blockIdx.x + 1) / p.ranges;
@@ -357,7 +368,7 @@ __global__ void __launch_bounds__(kThreadsR, rows_per_sm<D, HT>()) masked_rows_k
     item += local;
     while (x < x1) {
         const int take = static_cast<int>(min(static_cast<int64_t>(w - t), x1 - x));
-        rows_item<T, D, HT>(p, sm, sr, seq, local, t, t + take, take == w, blockIdx.x + item);
+        rows_item<T, D, HT, kWarps>(p, sm, sr, seq, local, t, t + take, take == w, blockIdx.x + item);
         x += take;
         t = 0;
         ++local;
@@ -446,16 +457,17 @@ template <typename T, int D, int HT>
 int launch_rows(p3d_ctx *ctx, MaskedParams p) {
     const int64_t items = p.max_q * p.kv_heads * p.head_tiles;  // of the longest sequence
     if (p.ranges > 0) {
-        P3D_CUDA(ctx, launch_pdl(masked_rows_kernel<T, D, HT>, dim3(p.ranges), dim3(kThreadsR), 0, ctx->stream, p));
-        const int rc = check_launch(ctx, "masked_rows");
+        P3D_CUDA(ctx, launch_pdl(masked_ranges_kernel<T, D, HT>, dim3(p.ranges), dim3(kThreadsR), 0, ctx->stream, p));
+        const int rc = check_launch(ctx, "masked_ranges");
         if (rc) return rc;
         P3D_CUDA(ctx, launch_pdl(masked_join_kernel<T, D>, dim3(static_cast<unsigned>(p.max_q * p.heads), p.nseq), dim3(kThreadsR), 0,
                                  ctx->stream, p));
         return check_launch(ctx, "masked_join");
     }
     if (items >= (int64_t(1) << 31)) return set_error(ctx, P3D_ERR_UNSUPPORTED, "p3d_masked_attention: too many query rows");
-    P3D_CUDA(ctx, launch_pdl(masked_rows_kernel<T, D, HT>, dim3(static_cast<unsigned>(items), p.nseq), dim3(kThreadsR), 0, ctx->stream, p));
-    return check_launch(ctx, "masked_rows");
+    P3D_CUDA(ctx, launch_pdl(masked_items_kernel<T, D, HT>, dim3(static_cast<unsigned>(items), p.nseq),
+                             dim3(32 * item_warps<D, HT>()), 0, ctx->stream, p));
+    return check_launch(ctx, "masked_items");
 }
 
 template <typename T, int D>
@@ -466,7 +478,7 @@ int launch_heads(p3d_ctx *ctx, const MaskedParams &p) {
 }  // namespace
 
 // Up to 512 keys an item is one block's (a cut and its join cost 2.4 us: 300
-// keys, 16 heads 6.3 against 8.7 us), and so it is where there are items for
+// keys, 16 heads 5.8 against 8.7 us; at 1000 keys both take 11), and so it is where there are items for
 // four rounds of the GPU.  Otherwise as many ranges as blocks fit, each of at
 // least 12 tiles: one sequence of 16384 keys, 4 K/V heads 14.4 us with 16 and
 // 15.9 with 8; 2000 keys, 12 heads 10.2 us with 4, 10.7 with 8, 14.4 with 32.
