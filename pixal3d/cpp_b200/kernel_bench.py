@@ -24,6 +24,11 @@ Kernels (config-2 shapes unless noted):
   window     8^3 window partition + windowed attention, 21,766 x 12 heads (config 3)
   dconv      config-3 stage-2 conv, ~347k rows, 64 (32 padded) -> 32 channels
   euler      Euler/CFG update with guidance rescale, 21,766 x 8
+  qrows      row quantisation to 8-bit integers, 8,184 x 4096 f16
+  lin8       trunk MLP up-projection with GELU on 8-bit integers, 8,184 x 1024 -> 4096
+  rotary     rotary positions, 16,368 rows x 32 heads x 64, interleaved, f16
+  mattn      masked attention, 2 x 4,092 rows, 16 heads x 64, causal behind 1,029 prefix keys, scores capped
+  mtoken     masked attention of one token of 5 sequences of 16,381 keys, 32 heads x 128 over 8
 Each run is small enough for an ncu capture (a few hundred MB on the
 device) while its inputs exceed the 126 MB L2.  Prints one JSON line.
 """
@@ -268,6 +273,43 @@ def run(kernel: str, reps: int, chunk: int | None = None) -> dict:
         ms = _time(lambda: ops.euler_cfg_step(x, vp, vn, offs, 0.5, 0.46, 3.0, 0.7, 1e-5), reps)
         bytes_ = 4 * n * 8 * 4
         return {"kernel": kernel, "ms": ms, "gbs": bytes_ / ms / 1e6, "bytes": bytes_}
+    if kernel == "qrows":
+        m, k = 8184, 4096
+        x = torch.randn((m, k), device=dev, generator=g).to(h)
+        q, sc = ops.quantize_rows(x)
+        ms = _time(lambda: ops.quantize_rows(x, q, sc), reps)
+        return {"kernel": kernel, "ms": ms, "gbs": 3 * m * k / ms / 1e6, "bytes": 3 * m * k}
+    if kernel == "lin8":
+        m, k, n = 8184, C, 4 * C
+        x, xs = ops.quantize_rows(torch.randn((m, k), device=dev, generator=g))
+        w, ws = ops.quantize_rows(torch.randn((n, k), device=dev, generator=g) / math.sqrt(k))
+        b = torch.zeros(n, device=dev)
+        out = torch.empty((m, n), dtype=torch.bfloat16, device=dev)
+        ms = _time(lambda: ops.linear_i8(x, xs, w, ws, b, out=out, epilogue=L.EPI_GELU_TANH), reps)
+        return {"kernel": kernel, "ms": ms, "tops": 2.0 * m * n * k / ms / 1e9}
+    if kernel == "rotary":
+        n, heads = 16368, 32
+        x = torch.randn((n, heads * 64), device=dev, generator=g).to(h)
+        freqs, amp = ops.rotary_frequencies(64, device=dev)
+        out = torch.empty_like(x)
+        ms = _time(lambda: ops.rotary(x, freqs, heads, 64, layout="interleaved", amplitude=amp, out=out), reps)
+        return {"kernel": kernel, "ms": ms, "gbs": 4.0 * x.numel() / ms / 1e6}
+    if kernel == "mattn":
+        n, pre = 4092, 1029
+        qkv = torch.randn((2 * n, 3 * C), device=dev, generator=g).to(h)
+        cu = torch.tensor([0, n, 2 * n], dtype=torch.int32, device=dev)
+        prefix = torch.tensor([pre, pre], dtype=torch.int32, device=dev)
+        ms = _time(lambda: ops.masked_attention(qkv[:, :C], qkv[:, C:2 * C], qkv[:, 2 * C:], cu, cu, n, n, 16, 0.125, causal=True,
+                                                prefix=prefix, softcap=30.0), reps)
+        pairs = 2 * (pre * pre + (n - pre) * (n + pre + 1) // 2)
+        return {"kernel": kernel, "ms": ms, "tflops": 4.0 * C * pairs / ms / 1e9}
+    if kernel == "mtoken":
+        seqs, lk, kv = 5, 16381, 8
+        q = torch.randn((seqs, 32 * 128), device=dev, generator=g).to(torch.bfloat16)
+        k, v = (torch.randn((seqs * lk, kv * 128), device=dev, generator=g).to(torch.bfloat16) for _ in range(2))
+        cq = torch.arange(seqs + 1, dtype=torch.int32, device=dev)
+        ms = _time(lambda: ops.masked_attention(q, k, v, cq, cq * lk, 1, lk, 32, 128 ** -0.5, kv_heads=kv, causal=True), reps)
+        return {"kernel": kernel, "ms": ms, "gbs": 4.0 * k.numel() / ms / 1e6}
     raise SystemExit(f"unknown kernel {kernel}")
 
 
