@@ -1,5 +1,5 @@
-// C ABI entry of the masked attention (kernels in p3d_masked_rows.cu and
-// p3d_masked_fmha.cuh).
+// C ABI entry of the masked attention (kernels in p3d_masked_rows.cu,
+// p3d_masked_pieces.cu and p3d_masked_fmha.cuh).
 #include <algorithm>
 #include <cmath>
 
@@ -7,8 +7,7 @@
 
 namespace p3d {
 int masked_attention_rows(p3d_ctx *ctx, const MaskedParams &p, int head_dim, int dtype);
-// Ranges that the key tiles of `items` items are cut into, 0 for a block an item.
-int masked_rows_ranges(int64_t items, int64_t max_k, int group, int head_dim);
+int masked_attention_pieces(p3d_ctx *ctx, const MaskedParams &p, int head_dim, int dtype);
 int masked_tiles_bf16_64(p3d_ctx *ctx, const MaskedParams &p, int dtype);
 int masked_tiles_bf16_128(p3d_ctx *ctx, const MaskedParams &p, int dtype);
 int masked_tiles_f16_64(p3d_ctx *ctx, const MaskedParams &p, int dtype);
@@ -16,8 +15,11 @@ int masked_tiles_f16_128(p3d_ctx *ctx, const MaskedParams &p, int dtype);
 
 namespace {
 
-// Up to this many queries a sequence go to the kernel that takes them one by one.
-constexpr int64_t kFewRows = 8;
+// Up to this many queries a sequence go to the kernels for few rows; up to
+// this many keys, to the one that takes each query alone.
+constexpr int64_t kFewRows = 8, kFewKeys = 512;
+
+size_t align256(size_t b) { return (b + 255) / 256 * 256; }
 
 // Smallest and largest document number of every key block, a warp a block.
 __global__ void __launch_bounds__(256) doc_range_kernel(const MaskedParams p) {
@@ -45,18 +47,38 @@ int masked_attention_tiles(p3d_ctx *ctx, const MaskedParams &p, int head_dim, in
     return head_dim == 64 ? masked_tiles_f16_64(ctx, p, dtype) : masked_tiles_f16_128(ctx, p, dtype);
 }
 
-size_t align256(size_t b) { return (b + 255) / 256 * 256; }
-
-// Ranges of the rows kernel and the bytes of its parts' sums and (maximum, sum).
-int rows_parts(int nseq, int64_t max_q, int64_t max_k, int heads, int kv_heads, int head_dim, size_t &o, size_t &ml) {
-    const int group = heads / kv_heads, per = group > 8 ? 16 : 8;
-    const int64_t items = static_cast<int64_t>(nseq) * max_q * kv_heads * ceil_div(group, per);
-    const int ranges = masked_rows_ranges(items, max_k, group, head_dim);
-    const size_t parts = static_cast<size_t>(ranges + items) * per;
-    o = align256(parts * head_dim * sizeof(float));
-    ml = align256(parts * sizeof(float2));
-    return ranges;
-}
+// Few queries over long keys: rows of an item (8, 16, 24 or 32 of the K/V
+// head's queries and heads), 16-key tiles of a piece, blocks, pieces at most,
+// and the bytes of their results.
+struct PiecePlan {
+    int item_rows, piece, blocks;
+    int64_t parts;
+    size_t o, ml;
+    PiecePlan(int nseq, int64_t max_q, int64_t max_k, int64_t rows_k, int heads, int kv_heads, int head_dim) {
+        const int64_t rows = std::max<int64_t>(max_q * (heads / kv_heads), 1);
+        // more rows of 128 dims would not stay in registers
+        item_rows = static_cast<int>(std::min<int64_t>(ceil_div(rows, 8) * 8, head_dim == 64 ? 32 : 16));
+        const int64_t items = kv_heads * ceil_div(rows, item_rows);  // of a sequence
+        const int64_t tiles = std::max<int64_t>(1, ceil_div(std::min(rows_k, nseq * max_k) / nseq, 16));  // of a mean item
+        // The fewest rounds of the 148 blocks times a piece's length and its own
+        // cost, over pieces of whole stages (the own cost taken as 8 tiles, not
+        // 32: 5 sequences of up to 16381 keys, 32 heads over 8 55.3 against
+        // 52.4 us; at least five rounds, for uneven lengths: 58.7).
+        int64_t best = 0;
+        piece = 16;
+        for (int64_t l = 16; l < tiles + 16; l += std::max<int64_t>(16, l / 8 / 16 * 16)) {
+            const int64_t cost = ceil_div(nseq * items * ceil_div(tiles, l), 148) * (l + 32);
+            if (best == 0 || cost < best) {
+                best = cost;
+                piece = static_cast<int>(l);
+            }
+        }
+        blocks = static_cast<int>(std::min<int64_t>(148, nseq * items * ceil_div(std::max<int64_t>(max_k, 1), 16 * static_cast<int64_t>(piece))));
+        parts = items * ((rows_k / 16 + nseq) / piece + nseq);
+        o = align256(static_cast<size_t>(parts) * item_rows * head_dim * sizeof(float));
+        ml = align256(static_cast<size_t>(parts) * item_rows * sizeof(float2));
+    }
+};
 
 }  // namespace
 }  // namespace p3d
@@ -67,8 +89,9 @@ extern "C" size_t p3d_masked_attention_workspace(int nseq, int64_t max_q, int64_
                                                  int heads, int kv_heads, int head_dim, int documents) {
     if (nseq <= 0 || max_q <= 0 || max_k < 0 || rows_q <= 0 || rows_k < 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
     if (max_q > kFewRows) return documents ? align256(static_cast<size_t>(rows_k / 64 + nseq + 1) * sizeof(int2)) : 0;
-    size_t o, ml;
-    return rows_parts(nseq, max_q, max_k, heads, kv_heads, head_dim, o, ml) ? o + ml : 0;
+    if (max_k <= kFewKeys) return 0;
+    const PiecePlan plan(nseq, max_q, max_k, rows_k, heads, kv_heads, head_dim);
+    return plan.o + plan.ml;
 }
 
 extern "C" int p3d_masked_attention(p3d_ctx *ctx, const void *q, int64_t ldq, const void *k, int64_t ldk, const void *v,
@@ -141,10 +164,13 @@ extern "C" int p3d_masked_attention(p3d_ctx *ctx, const void *q, int64_t ldq, co
         p.doc_range = static_cast<int2 *>(ws);
         return masked_attention_tiles(ctx, p, head_dim, dtype);
     }
-    size_t o, ml;
-    p.head_tiles = static_cast<int>(ceil_div(p.group, p.group > 8 ? 16 : 8));
-    p.ranges = rows_parts(nseq, max_q, max_k, heads, kv_heads, head_dim, o, ml);
+    if (max_k <= kFewKeys) return masked_attention_rows(ctx, p, head_dim, dtype);
+    const PiecePlan plan(nseq, max_q, max_k, rows_k, heads, kv_heads, head_dim);
+    p.item_rows = plan.item_rows;
+    p.piece = plan.piece;
+    p.blocks = plan.blocks;
+    p.parts = plan.parts;
     p.part_o = static_cast<float *>(ws);
-    p.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(ws) + o);
-    return masked_attention_rows(ctx, p, head_dim, dtype);
+    p.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(ws) + plan.o);
+    return masked_attention_pieces(ctx, p, head_dim, dtype);
 }

@@ -18,10 +18,12 @@ struct MaskedParams {
     int causal;
     const int32_t *prefix, *doc_q, *doc_k;
     const float *slopes;
-    // the rows kernel: groups of 8 or 16 heads of a K/V head; equal ranges the
-    // key tiles are cut into (0: a block an item), and the parts' sums [part]
-    // [8 or 16 heads][D] against their own maxima, [part][heads] (maximum, sum)
-    int head_tiles, ranges;
+    int head_tiles;  // few keys: groups of 8 or 16 heads of a K/V head
+    // few queries, long keys: rows (query, head) of an item, key tiles of a
+    // piece, blocks, and the pieces' results: [parts][item_rows][D] sums
+    // against their own maxima, and (maximum, sum)
+    int item_rows, piece, blocks;
+    int64_t parts;
     float *part_o;
     float2 *part_ml;
     int2 *doc_range; // (smallest, largest) document number of every 64-key block

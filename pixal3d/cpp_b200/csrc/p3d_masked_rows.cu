@@ -1,12 +1,11 @@
-// Masked attention for few query rows: one query of each sequence at a time,
-// its keys split over warps and blocks and joined.
+// Masked attention for few query rows over few keys: a block takes one query
+// and one K/V head with the (up to 16) query heads that share it; its warps
+// take 16-key tiles in turn, each with its own running maximum and sum, and
+// are joined in shared memory.  (Long keys: p3d_masked_pieces.cu.)
 //
-// With one new token a sequence the work is reading K and V once: 2 d bytes a
-// key and shared head, at 4 d operations for each of its heads.  A block takes
-// one query, one K/V head with the (up to 16) query heads that share it, and
-// one range of keys; its 4 warps take 16-key tiles in turn, each with its own
-// running maximum and sum, and are joined in shared memory; the blocks of a
-// query are joined by a second kernel.
+// A call is a chain of memory latencies rather than bytes: 300 keys, 16 heads
+// of 64 take 5.8 us, 8 sequences of 500 keys 7.1; with 4 warps instead of 8
+// they took 6.6 and 9.4.
 //
 // All heads of a block see the same keys, so a hidden key's V is never read
 // (zeros stand in), whatever it holds.
@@ -25,86 +24,10 @@
 // and g + 8.
 #include <algorithm>
 
-#include "p3d_masked.cuh"
+#include "p3d_masked_small.cuh"
 
 namespace p3d {
 namespace {
-
-constexpr int kWarps = 4;  // of a block that walks a range, and of the join
-constexpr int kThreadsR = 32 * kWarps;
-// A block that takes a whole item of few keys has 8 warps: half as many tiles
-// one after the other.
-
-template <typename T>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
-
-__device__ __forceinline__ uint32_t word(const uint4 &u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; }
-
-// Key tiles of one item of a sequence (at least one, so that every item has a
-// block) and the sequence's items: query, K/V head, 8 * HT of its heads.
-__device__ __forceinline__ int item_tiles(const SeqRange &sr) { return max(1, (sr.lk + 15) / 16); }
-__device__ __forceinline__ int seq_items(const MaskedParams &p, const SeqRange &sr) {
-    return static_cast<int>(min(static_cast<int64_t>(sr.lq), p.max_q)) * p.kv_heads * p.head_tiles;
-}
-
-// The tiles of all items (a whole warp calls it).
-__device__ __forceinline__ int64_t all_tiles(const MaskedParams &p, int lane) {
-    int64_t t = 0;
-    for (int s = lane; s < p.nseq; s += 32) {
-        const SeqRange sr = seq_range(p, s);
-        t += static_cast<int64_t>(item_tiles(sr)) * seq_items(p, sr);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    return t;
-}
-
-// Tiles and items of the sequences before `seq`, or, with seq < 0, of those
-// before the one that holds tile x, whose number is returned.
-__device__ __forceinline__ int find_seq(const MaskedParams &p, int lane, int seq, int64_t x, int64_t &tiles, int64_t &items) {
-    tiles = items = 0;
-    for (int c = 0; c < p.nseq; c += 32) {
-        int64_t w = 0, n = 0;
-        if (c + lane < p.nseq) {
-            const SeqRange sr = seq_range(p, c + lane);
-            n = seq_items(p, sr);
-            w = n * item_tiles(sr);
-        }
-        int64_t wi = w, ni = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t a = __shfl_up_sync(0xffffffffu, wi, o), b = __shfl_up_sync(0xffffffffu, ni, o);
-            if (lane >= o) {
-                wi += a;
-                ni += b;
-            }
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, seq >= 0 ? c + lane == seq : tiles + wi > x);
-        if (hit) {
-            const int l = __ffs(hit) - 1;
-            tiles += __shfl_sync(0xffffffffu, wi - w, l);
-            items += __shfl_sync(0xffffffffu, ni - n, l);
-            return c + l;
-        }
-        tiles += __shfl_sync(0xffffffffu, wi, 31);
-        items += __shfl_sync(0xffffffffu, ni, 31);
-    }
-    return p.nseq;
-}
 
 template <int D, int HT, int W>
 struct RowsShared {
@@ -112,12 +35,9 @@ struct RowsShared {
     float m[W][8 * HT], l[W][8 * HT];
 };
 
-// One item's key tiles [t0, t1): item `local` of sequence seq.  Writes the
-// output when `whole`, else the part `slot` (sums against its own maximum).
-// HT: 8 heads a block, or 16.
+// Item `local` (query, K/V head, group of 8 HT of its heads) of sequence seq.
 template <typename T, int D, int HT, int W>
-__device__ __forceinline__ void rows_item(const MaskedParams &p, RowsShared<D, HT, W> &sm, const SeqRange &sr, int seq, int local, int t0,
-                                          int t1, bool whole, int64_t slot) {
+__device__ __forceinline__ void rows_item(const MaskedParams &p, RowsShared<D, HT, W> &sm, const SeqRange &sr, int seq, int local) {
     constexpr int KC = D / 32;  // 16-byte chunks of a K row per lane
     constexpr int VS = D / 64;  // 64-dim slabs of V
     constexpr int H = 8 * HT;
@@ -130,7 +50,7 @@ __device__ __forceinline__ void rows_item(const MaskedParams &p, RowsShared<D, H
     const int docq = p.doc_q ? p.doc_q[qrow] : 0;
     const int head0 = hk * p.group + ht * H;
     const int nrows = min(H, p.group - ht * H);
-    const int tile0 = t0, tile1 = min(t1, (max(end, 0) + 15) / 16);
+    const int tiles = (max(end, 0) + 15) / 16;
 
     const T *kb = static_cast<const T *>(p.k) + sr.k0 * p.ldk + hk * D;
     const T *vb = static_cast<const T *>(p.v) + sr.k0 * p.ldv + hk * D;
@@ -145,7 +65,7 @@ __device__ __forceinline__ void rows_item(const MaskedParams &p, RowsShared<D, H
                 kf[t][c] = __ldg(reinterpret_cast<const uint4 *>(kb + key * p.ldk + c * 32 + j * 8));
         }
     };
-    if (tile0 + warp < tile1) load_k(tile0 + warp);
+    if (warp < tiles) load_k(warp);
 
     uint4 qf[HT][KC];
 #pragma unroll
@@ -176,21 +96,7 @@ __device__ __forceinline__ void rows_item(const MaskedParams &p, RowsShared<D, H
         l[r] = 0.0f;
     }
 
-    // With 128-byte rows the tile after the next is fetched into L2, a line a
-    // lane (16 sequences of up to 8192 keys, 16 heads: 98 -> 82 us); with
-    // 256-byte rows the registers' own loads keep enough in flight and the same
-    // made it slower (99 -> 106 us).
-    auto prefetch = [&](int tile) {
-        constexpr int LINES = D / 64;  // of a row
-        const int key = min(tile * 16 + lane / LINES % 16, sr.lk - 1);
-        if (LINES == 2 || lane < 16) prefetch_l2(kb + key * p.ldk + lane % LINES * 64);
-        if (LINES == 2 || lane >= 16) prefetch_l2(vb + key * p.ldv + lane % LINES * 64);
-    };
-    constexpr int kAhead = D == 64 ? 2 : 0;
-    for (int a = 1; a < kAhead; ++a)
-        if (tile0 + warp + a * W < tile1) prefetch(tile0 + warp + a * W);
-    for (int tile = tile0 + warp; tile < tile1; tile += W) {
-        if (kAhead > 0 && tile + kAhead * W < tile1) prefetch(tile + kAhead * W);
+    for (int tile = warp; tile < tiles; tile += W) {
         bool vis[4];
         uint4 vf[4][VS];
 #pragma unroll
@@ -215,7 +121,7 @@ __device__ __forceinline__ void rows_item(const MaskedParams &p, RowsShared<D, H
                     mma16816<T>(sc[t], a, word(kf[t][c], 2 * h), word(kf[t][c], 2 * h + 1));
                 }
         }
-        if (tile + W < tile1) load_k(tile + W);
+        if (tile + W < tiles) load_k(tile + W);
         float mx[HT];
         bool raised = false;
 #pragma unroll
@@ -280,7 +186,6 @@ __device__ __forceinline__ void rows_item(const MaskedParams &p, RowsShared<D, H
             }
     }
     // join the warps
-    __syncthreads();  // the last item's parts have been read
 #pragma unroll
     for (int r = 0; r < HT; ++r) {
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -317,21 +222,10 @@ __device__ __forceinline__ void rows_item(const MaskedParams &p, RowsShared<D, H
             oo.z = fmaf(x.z, a, oo.z);
             oo.w = fmaf(x.w, a, oo.w);
         }
-        if (whole) {
-            const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-            *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + qrow * p.ldo + static_cast<int64_t>(head0 + r) * D + d) =
-                make_uint2(pack2<T>(oo.x * inv, oo.y * inv), pack2<T>(oo.z * inv, oo.w * inv));
-        } else {
-            *reinterpret_cast<float4 *>(p.part_o + (slot * H + r) * D + d) = oo;
-            if (d == 0) p.part_ml[slot * H + r] = make_float2(mm, ll);
-        }
+        const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+        *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + qrow * p.ldo + static_cast<int64_t>(head0 + r) * D + d) =
+            make_uint2(pack2<T>(oo.x * inv, oo.y * inv), pack2<T>(oo.z * inv, oo.w * inv));
     }
-}
-
-// Blocks an SM holds at once (registers).
-template <int D, int HT>
-constexpr int rows_per_sm() {
-    return (D == 64 ? 4 : 3) - (HT - 1);
 }
 
 template <int D, int HT>
@@ -345,125 +239,13 @@ __global__ void __launch_bounds__(32 * item_warps<D, HT>()) masked_items_kernel(
     pdl_wait();
     pdl_trigger();
     const SeqRange sr = seq_range(p, blockIdx.y);
-    if (static_cast<int>(blockIdx.x) < seq_items(p, sr))
-        rows_item<T, D, HT, W>(p, sm, sr, blockIdx.y, blockIdx.x, 0, item_tiles(sr), true, 0);
+    if (blockIdx.x < min(static_cast<int64_t>(sr.lq), p.max_q) * p.kv_heads * p.head_tiles)
+        rows_item<T, D, HT, W>(p, sm, sr, blockIdx.y, blockIdx.x);
 }
 
 template <typename T, int D, int HT>
-__global__ void __launch_bounds__(kThreadsR, rows_per_sm<D, HT>()) masked_ranges_kernel(const MaskedParams p) {
-    __shared__ RowsShared<D, HT, kWarps> sm;
-    pdl_wait();
-    pdl_trigger();
-    const int lane = threadIdx.x & 31;
-    const int64_t total = all_tiles(p, lane);  // every warp finds the same
-    int64_t x = total * blockIdx.x / p.ranges;
-    const int64_t x1 = total * (blockIdx.x + 1) / p.ranges;
-    if (x >= x1) return;
-    int64_t before, item;
-    int seq = find_seq(p, lane, -1, x, before, item);
-    if (seq >= p.nseq) return;
-    SeqRange sr = seq_range(p, seq);
-    int w = item_tiles(sr);
-    int local = static_cast<int>((x - before) / w), t = static_cast<int>((x - before) % w);
-    item += local;
-    while (x < x1) {
-        const int take = static_cast<int>(min(static_cast<int64_t>(w - t), x1 - x));
-        rows_item<T, D, HT, kWarps>(p, sm, sr, seq, local, t, t + take, take == w, blockIdx.x + item);
-        x += take;
-        t = 0;
-        ++local;
-        ++item;
-        while (x < x1 && local >= seq_items(p, sr) && seq + 1 < p.nseq) {
-            sr = seq_range(p, ++seq);
-            w = item_tiles(sr);
-            local = 0;
-        }
-    }
-}
-
-// A block joins the parts of one query row and head.  Part number: block +
-// item, which no other (block, item) pair has, as the items a block meets
-// begin where the last block's end.
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreadsR) masked_join_kernel(const MaskedParams p) {
-    constexpr int E = D / 32;
-    __shared__ float so[kWarps][D];
-    __shared__ float2 sml[kWarps];
-    pdl_wait();
-    pdl_trigger();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int head = blockIdx.x % p.heads, qi = blockIdx.x / p.heads, seq = blockIdx.y;
-    const SeqRange sr = seq_range(p, seq);
-    if (qi >= sr.lq) return;
-    const int H = p.group > 8 ? 16 : 8;
-    const int in = head % p.group, local = (qi * p.kv_heads + head / p.group) * p.head_tiles + in / H, r = in % H;
-    const int64_t total = all_tiles(p, lane);
-    int64_t first, item;
-    find_seq(p, lane, seq, 0, first, item);
-    const int w = item_tiles(sr);
-    first += static_cast<int64_t>(local) * w;
-    item += local;
-    // tile x lies in range ((x + 1) ranges - 1) / total
-    const int64_t b0 = ((first + 1) * p.ranges - 1) / total, b1 = ((first + w) * p.ranges - 1) / total;
-    if (b0 == b1) return;  // one block had all of it
-    const int64_t s0 = b0 + item, s1 = b1 + item;
-    float mm = -INFINITY;
-    for (int64_t s = s0 + threadIdx.x % 32 * kWarps + warp; s <= s1; s += 32 * kWarps) mm = fmaxf(mm, p.part_ml[s * H + r].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-    const float base = mm == -INFINITY ? 0.0f : mm;
-    float ll = 0.0f, oo[E] = {};
-#pragma unroll 8
-    for (int64_t s = s0 + warp; s <= s1; s += kWarps) {
-        const float2 ml = p.part_ml[s * H + r];
-        const float a = ex2f(ml.x - base);
-        ll = fmaf(ml.y, a, ll);
-        const float *src = p.part_o + (s * H + r) * D + lane * E;
-        float v[E];
-        if constexpr (E == 4) {
-            const float4 f = *reinterpret_cast<const float4 *>(src);
-            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-        } else {
-            const float2 f = *reinterpret_cast<const float2 *>(src);
-            v[0] = f.x, v[1] = f.y;
-        }
-#pragma unroll
-        for (int e = 0; e < E; ++e) oo[e] = fmaf(v[e], a, oo[e]);
-    }
-    if (lane == 0) sml[warp] = make_float2(mm, ll);
-#pragma unroll
-    for (int e = 0; e < E; ++e) so[warp][lane * E + e] = oo[e];
-    __syncthreads();
-    if (threadIdx.x * 2 < D) {
-        const int d = threadIdx.x * 2;
-        float top = -INFINITY, sum = 0.0f, y0 = 0.0f, y1 = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kWarps; ++k) top = fmaxf(top, sml[k].x);
-        const float b = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-        for (int k = 0; k < kWarps; ++k) {
-            const float a = ex2f(sml[k].x - b);
-            sum = fmaf(sml[k].y, a, sum);
-            y0 = fmaf(so[k][d], a, y0);
-            y1 = fmaf(so[k][d + 1], a, y1);
-        }
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        *reinterpret_cast<uint32_t *>(static_cast<T *>(p.out) + (sr.q0 + static_cast<int64_t>(qi)) * p.ldo +
-                                      static_cast<int64_t>(head) * D + d) = pack2<T>(y0 * inv, y1 * inv);
-    }
-}
-
-template <typename T, int D, int HT>
-int launch_rows(p3d_ctx *ctx, MaskedParams p) {
+int launch_rows(p3d_ctx *ctx, const MaskedParams &p) {
     const int64_t items = p.max_q * p.kv_heads * p.head_tiles;  // of the longest sequence
-    if (p.ranges > 0) {
-        P3D_CUDA(ctx, launch_pdl(masked_ranges_kernel<T, D, HT>, dim3(p.ranges), dim3(kThreadsR), 0, ctx->stream, p));
-        const int rc = check_launch(ctx, "masked_ranges");
-        if (rc) return rc;
-        P3D_CUDA(ctx, launch_pdl(masked_join_kernel<T, D>, dim3(static_cast<unsigned>(p.max_q * p.heads), p.nseq), dim3(kThreadsR), 0,
-                                 ctx->stream, p));
-        return check_launch(ctx, "masked_join");
-    }
     if (items >= (int64_t(1) << 31)) return set_error(ctx, P3D_ERR_UNSUPPORTED, "p3d_masked_attention: too many query rows");
     P3D_CUDA(ctx, launch_pdl(masked_items_kernel<T, D, HT>, dim3(static_cast<unsigned>(items), p.nseq),
                              dim3(32 * item_warps<D, HT>()), 0, ctx->stream, p));
@@ -471,23 +253,12 @@ int launch_rows(p3d_ctx *ctx, MaskedParams p) {
 }
 
 template <typename T, int D>
-int launch_heads(p3d_ctx *ctx, const MaskedParams &p) {
+int launch_heads(p3d_ctx *ctx, MaskedParams p) {
+    p.head_tiles = static_cast<int>(ceil_div(p.group, p.group > 8 ? 16 : 8));
     return p.group > 8 ? launch_rows<T, D, 2>(ctx, p) : launch_rows<T, D, 1>(ctx, p);
 }
 
 }  // namespace
-
-// Up to 512 keys an item is one block's (a cut and its join cost 2.4 us: 300
-// keys, 16 heads 5.8 against 8.7 us; at 1000 keys both take 11), and so it is where there are items for
-// four rounds of the GPU.  Otherwise as many ranges as blocks fit, each of at
-// least 12 tiles: one sequence of 16384 keys, 4 K/V heads 14.4 us with 16 and
-// 15.9 with 8; 2000 keys, 12 heads 10.2 us with 4, 10.7 with 8, 14.4 with 32.
-int masked_rows_ranges(int64_t items, int64_t max_k, int group, int head_dim) {
-    const int64_t tiles = ceil_div(max_k, 16);
-    const int64_t capacity = 148 * ((head_dim == 64 ? 4 : 3) - (group > 8 ? 1 : 0));
-    if (tiles <= 32 || items >= 4 * capacity) return 0;
-    return static_cast<int>(std::max<int64_t>(1, std::min(capacity, items * tiles / 12)));
-}
 
 int masked_attention_rows(p3d_ctx *ctx, const MaskedParams &p, int head_dim, int dtype) {
     if (dtype == P3D_BF16)

@@ -314,3 +314,64 @@ def test_refusals():
             bad()
         assert e.value.status == status
     assert o.masked_attention(q[:0], q, q, c, c, 4, 4, 2, 1.0).shape == (0, 128)
+
+
+LONG = [[(1, 3000)], [(1, 700), (1, 0), (2, 5000), (8, 513)], [(5, 1200), (0, 900), (3, 2)], [(2, 4100)] * 5, [(1, 600)] * 40, [(8, 2000), (8, 5)]]
+
+
+@pytest.mark.parametrize("d,dtype", [(64, HF), (128, BF)])
+@pytest.mark.parametrize("heads,kv_heads", [(4, 4), (8, 2), (12, 1), (40, 1)])
+@pytest.mark.parametrize("lens", LONG)
+def test_few_queries_over_long_keys(lens, heads, kv_heads, d, dtype):
+    """Up to 8 queries a sequence over keys that are shared out over the GPU:
+    items of 8 to 32 rows and more, whole and cut ones."""
+    run(lens, heads, kv_heads, d, dtype, causal=True, spare=5)
+    run(lens, heads, kv_heads, d, dtype, slopes=torch.rand(heads, device="cuda") * 0.01, softcap=20.0)
+
+
+@pytest.mark.parametrize("d,dtype", [(64, HF), (128, BF)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("value", [0.0, math.nan, math.inf])
+def test_few_queries_over_long_keys_masked(d, dtype, causal, value):
+    lens = [(1, 900), (4, 1500), (8, 640), (3, 1)]
+    g = torch.Generator(device="cuda").manual_seed(11)
+    nq, nk = sum(a for a, _ in lens), sum(b for _, b in lens)
+    dk = torch.randint(0, 3, (nk,), device="cuda", generator=g).int()
+    dk[::5] = 99  # nobody's
+    dq = torch.randint(0, 4, (nq,), device="cuda", generator=g).int()  # 3 has no key
+    prefix = torch.tensor([0, 100, 640, 1], dtype=torch.int32, device="cuda")
+
+    def hide(hidden):
+        def poison(q, k, v):
+            if value != 0.0:
+                k[hidden.nonzero().flatten()] = value
+                v[hidden.nonzero().flatten()] = value
+        return poison
+    run(lens, 8, 2, d, dtype, causal=causal, doc_q=dq, doc_k=dk, poison=hide(dk == 99))
+    at = torch.cat([torch.arange(b) for _, b in lens]).cuda()
+    shared = at < torch.cat([prefix[i].repeat(b) for i, (_, b) in enumerate(lens)])
+    run(lens, 8, 2, d, dtype, causal=causal, doc_q=dq, doc_k=dk, prefix=prefix, slopes=torch.rand(8, device="cuda") * 0.01,
+        poison=hide((dk == 99) & ~shared))
+
+
+@pytest.mark.parametrize("d,dtype", [(64, HF), (128, BF)])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_later_keys_of_few_queries(d, dtype, value):
+    """Of the last keys some queries see a non-finite value and others do not."""
+    n, lq = 1000, 6
+    got = {}
+    for bad in (False, True):
+        g = torch.Generator(device="cuda").manual_seed(3)
+        q = torch.randn((lq, 4 * d), device="cuda", generator=g).to(dtype)
+        k, v = (torch.randn((n, 2 * d), device="cuda", generator=g).to(dtype) for _ in range(2))
+        if bad:
+            v[n - 3, 3] = value  # seen from query 3 on
+            v[n - 2, d + d - 1] = -value
+        got[bad] = ops().masked_attention(q, k, v, cu([lq]), cu([n]), lq, n, 4, 0.1, kv_heads=2, causal=True)
+    want = got[False].clone()
+    want[3:, 3] = want[3:, d + 3] = value
+    want[4:, 3 * d - 1] = want[4:, 4 * d - 1] = -value
+    ok = want.isfinite()
+    assert torch.equal(got[True].isfinite(), ok) and torch.equal(got[True].isnan(), want.isnan())
+    assert torch.equal(got[True][~ok].nan_to_num(7.5, 1e4, -1e4), want[~ok].nan_to_num(7.5, 1e4, -1e4))
+    assert torch.equal(got[True][ok], want[ok])
