@@ -61,12 +61,15 @@ struct PiecePlan {
         const int64_t items = kv_heads * ceil_div(rows, item_rows);  // of a sequence
         const int64_t tiles = std::max<int64_t>(1, ceil_div(std::min(rows_k, nseq * max_k) / nseq, 16));  // of a mean item
         // The fewest rounds of the 148 blocks times a piece's length and its own
-        // cost, over pieces of whole stages (the own cost taken as 8 tiles, not
-        // 32: 5 sequences of up to 16381 keys, 32 heads over 8 55.3 against
-        // 52.4 us; at least five rounds, for uneven lengths: 58.7).
+        // cost, over pieces of whole stages and no longer than a block's even
+        // share, so that uneven sequences end together (4 sequences of up to
+        // 16000 keys, 5 queries 89 against 122 us without that bound; the own
+        // cost taken as 8 tiles, not 32: 5 sequences of up to 16381 keys, 32
+        // heads over 8 55.3 against 52.4 us).
+        const int64_t share = std::max<int64_t>(nseq * items * tiles / 148, 16);
         int64_t best = 0;
         piece = 16;
-        for (int64_t l = 16; l < tiles + 16; l += std::max<int64_t>(16, l / 8 / 16 * 16)) {
+        for (int64_t l = 16; l < std::min(tiles, share) + 16; l += std::max<int64_t>(16, l / 8 / 16 * 16)) {
             const int64_t cost = ceil_div(nseq * items * ceil_div(tiles, l), 148) * (l + 32);
             if (best == 0 || cost < best) {
                 best = cost;
