@@ -25,6 +25,10 @@
 // and at the end each query adds the noted blocks' non-finite values that it
 // does see.  Blocks that every query sees need none of this.
 //
+// Few CTAs over long keys: the visits are cut into splits, whose sums against
+// their own maxima a second kernel joins (one sequence of 64 queries, 16 heads
+// of 64, 8192 keys: SPLITOFF us without, SPLITON with).
+//
 // Rows past the sequence's end compute on whatever the tile holds and are not
 // stored.  Every wait is bounded.
 #include <type_traits>
@@ -159,7 +163,8 @@ __global__ void __launch_bounds__(kThreadsF, 2)
     constexpr int ST = C::STAGES;
     pdl_wait();
     const int head = blockIdx.x, seq = blockIdx.y;
-    const int tile = p.causal ? gridDim.z - 1 - blockIdx.z : blockIdx.z;  // the longest rows first
+    const int split = blockIdx.z % p.splits, z = blockIdx.z / p.splits;
+    const int tile = p.causal ? gridDim.z / p.splits - 1 - z : z;  // the longest rows first
     const SeqRange sr = seq_range(p, seq);
     const int row0 = tile * kM;                       // first query of the tile, within the sequence
     const int nrows = min(min(sr.lq, static_cast<int>(p.max_q)) - row0, kM);
@@ -215,7 +220,9 @@ __global__ void __launch_bounds__(kThreadsF, 2)
     const int limit = p.causal ? min(sr.lk, max(pre, pos_hi + 1)) : sr.lk;  // no query of the tile sees a key from here on
     const int blocks = max(0, (limit + kN - 1) / kN);
     int qdoc_lo = 0, qdoc_hi = 0;
-    int chunk = 0;
+    // this split's share of the visits
+    int chunk = static_cast<int>(static_cast<int64_t>(blocks) * split / p.splits);
+    const int visits = static_cast<int>(static_cast<int64_t>(blocks) * (split + 1) / p.splits);
     uint32_t seen = 0, mixed = 0;
     // The order of the visits.  Under a distance bias the scores of most rows
     // fall away from their own position, so the tile's own block comes first,
@@ -224,7 +231,7 @@ __global__ void __launch_bounds__(kThreadsF, 2)
     const int own_block = BIAS ? min(blocks - 1, max(0, pos_hi / kN)) : -1;
     auto block_at = [&](int visit) { return visit <= own_block ? own_block - visit : visit; };
     auto classify = [&]() {
-        const bool in = chunk + lane < blocks;
+        const bool in = chunk + lane < visits;
         const int blk = block_at(chunk + lane), kb = blk * kN;
         int dlo = 0, dhi = 0;
         if (DOCS && in) {
@@ -242,7 +249,7 @@ __global__ void __launch_bounds__(kThreadsF, 2)
     auto next_block = [&](bool &is_mixed) -> int {  // the next block to visit, or -1
         while (seen == 0) {
             chunk += 32;
-            if (chunk >= blocks) return -1;
+            if (chunk >= visits) return -1;
             classify();
         }
         const int l = __ffs(seen) - 1;
@@ -263,7 +270,7 @@ __global__ void __launch_bounds__(kThreadsF, 2)
             qdoc_lo = __reduce_min_sync(0xffffffffu, lo);
             qdoc_hi = __reduce_max_sync(0xffffffffu, hi);
         }
-        if (blocks > 0) {
+        if (chunk < visits) {
             classify();
             cur = next_block(cur_mixed);
         }
@@ -277,7 +284,10 @@ __global__ void __launch_bounds__(kThreadsF, 2)
     const bool nothing = *any_seen == 0;
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
 
-    if (nothing) {
+    if (nothing && p.splits > 1) {
+        for (int e = threadIdx.x; e < nrows; e += kThreadsF)
+            p.part_ml[((sr.q0 + static_cast<int64_t>(row0) + e) * p.heads + head) * p.splits + split] = make_float2(-INFINITY, 0.0f);
+    } else if (nothing) {
         T *o = static_cast<T *>(p.out) + (sr.q0 + static_cast<int64_t>(row0)) * p.ldo + static_cast<int64_t>(head) * D;
         for (int e = threadIdx.x; e < nrows * (D / 8); e += kThreadsF)
             *reinterpret_cast<uint4 *>(o + (e / (D / 8)) * p.ldo + e % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
@@ -521,7 +531,9 @@ __global__ void __launch_bounds__(kThreadsF, 2)
         float l0, l1;
         l2.get(l0, l1);
         const float l = l0 + l1;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = p.splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+        const int64_t part = ((sr.q0 + static_cast<int64_t>(row0) + row) * p.heads + head) * p.splits + split;
+        if (p.splits > 1 && ok && valid) p.part_ml[part] = make_float2(m_run, l);
         const int bad0 = bad[0], bad1 = bad[1];
         T *dst = static_cast<T *>(p.out) + (sr.q0 + static_cast<int64_t>(row0) + row) * p.ldo + static_cast<int64_t>(head) * D;
 #pragma unroll 1
@@ -542,6 +554,12 @@ __global__ void __launch_bounds__(kThreadsF, 2)
                     if (!isfinite(x)) o[e] += x;
                 }
             }
+            if (p.splits > 1) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 4)
+                    *reinterpret_cast<float4 *>(p.part_o + part * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                continue;
+            }
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
                 uint4 u;
@@ -560,6 +578,40 @@ __global__ void __launch_bounds__(kThreadsF, 2)
     if (warp == 1) tmem_dealloc(tmem, kTmemCols);
 }
 
+// A warp joins the splits of one query and head.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) masked_splits_kernel(const MaskedParams p) {
+    constexpr int E = D / 32;
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31;
+    const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    const int head = static_cast<int>(item % p.heads);
+    const int64_t qi = item / p.heads;
+    const SeqRange sr = seq_range(p, blockIdx.y);
+    if (qi >= sr.lq || qi >= p.max_q) return;
+    const int64_t at = ((sr.q0 + qi) * p.heads + head) * p.splits;
+    const float mine = lane < p.splits ? p.part_ml[at + lane].x : -INFINITY;
+    float mm = mine;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+    float ll = 0.0f, oo[E] = {};
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) {
+        const float2 ml = p.part_ml[at + s];
+        if (ml.x == -INFINITY) continue;  // saw nothing and wrote no sums
+        const float a = ex2f(ml.x - mm);
+        ll = fmaf(ml.y, a, ll);
+        const float *src = p.part_o + (at + s) * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) oo[e] = fmaf(src[e], a, oo[e]);
+    }
+    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+    T *dst = static_cast<T *>(p.out) + (sr.q0 + qi) * p.ldo + static_cast<int64_t>(head) * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t *>(dst + e) = pack2<T>(oo[e] * inv, oo[e + 1] * inv);
+}
+
 template <typename T, int D, bool CAP, bool BIAS, bool DOCS>
 int launch_fmha(p3d_ctx *ctx, const MaskedParams &p, int dtype) {
     CUtensorMap tq, tk, tv;
@@ -568,12 +620,16 @@ int launch_fmha(p3d_ctx *ctx, const MaskedParams &p, int dtype) {
         (rc = make_tmap_16bit_2d(ctx, &tv, p.v, dtype, p.rows_k, static_cast<uint64_t>(p.kv_heads) * D, p.ldv, kN)))
         return rc;
     const int64_t tiles = ceil_div(p.max_q, kM);
-    if (tiles > 65535) return set_error(ctx, P3D_ERR_UNSUPPORTED, "p3d_masked_attention: max_q above 8388480");
+    if (tiles * p.splits > 65535) return set_error(ctx, P3D_ERR_UNSUPPORTED, "p3d_masked_attention: max_q above 8388480");
     auto kernel = masked_fmha_kernel<T, D, CAP, BIAS, DOCS>;
     P3D_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-    P3D_CUDA(ctx, launch_pdl(kernel, dim3(p.heads, p.nseq, static_cast<unsigned>(tiles)), dim3(kThreadsF), kSmem, ctx->stream, tq,
-                             tk, tv, p));
-    return check_launch(ctx, "masked_fmha");
+    P3D_CUDA(ctx, launch_pdl(kernel, dim3(p.heads, p.nseq, static_cast<unsigned>(tiles * p.splits)), dim3(kThreadsF), kSmem, ctx->stream,
+                             tq, tk, tv, p));
+    rc = check_launch(ctx, "masked_fmha");
+    if (rc || p.splits == 1) return rc;
+    P3D_CUDA(ctx, launch_pdl(masked_splits_kernel<T, D>, dim3(static_cast<unsigned>(ceil_div(p.max_q * p.heads, 8)), p.nseq), dim3(256),
+                             0, ctx->stream, p));
+    return check_launch(ctx, "masked_splits");
 }
 
 template <typename T, int D, bool DOCS>

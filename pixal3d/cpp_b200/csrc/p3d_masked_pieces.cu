@@ -120,9 +120,10 @@ struct Walk {
     }
 };
 
+// Infinity or NaN in the low half.
 template <typename T>
-__device__ __forceinline__ bool odd16(uint32_t h) {  // infinity or NaN in the low half
-    constexpr uint32_t e = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+__device__ __forceinline__ bool odd16(uint32_t h) {
+    constexpr uint32_t e = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
     return (h & e) == e;
 }
 
@@ -558,12 +559,12 @@ int launch_pieces(p3d_ctx *ctx, const MaskedParams &p, int dtype) {
 
 template <typename T, int D>
 int launch_rows(p3d_ctx *ctx, const MaskedParams &p, int dtype) {
-    switch (p.item_rows / 8) {
-        case 1: return launch_pieces<T, D, 1>(ctx, p, dtype);
-        case 2: return launch_pieces<T, D, 2>(ctx, p, dtype);
-        case 3: return launch_pieces<T, D, 3>(ctx, p, dtype);
-        default: return launch_pieces<T, D, 4>(ctx, p, dtype);
+    if (p.item_rows == 8) return launch_pieces<T, D, 1>(ctx, p, dtype);
+    if constexpr (D == 64) {
+        if (p.item_rows == 24) return launch_pieces<T, D, 3>(ctx, p, dtype);
+        if (p.item_rows == 32) return launch_pieces<T, D, 4>(ctx, p, dtype);
     }
+    return launch_pieces<T, D, 2>(ctx, p, dtype);
 }
 
 }  // namespace

@@ -375,3 +375,22 @@ def test_later_keys_of_few_queries(d, dtype, value):
     assert torch.equal(got[True].isfinite(), ok) and torch.equal(got[True].isnan(), want.isnan())
     assert torch.equal(got[True][~ok].nan_to_num(7.5, 1e4, -1e4), want[~ok].nan_to_num(7.5, 1e4, -1e4))
     assert torch.equal(got[True][ok], want[ok])
+
+
+@pytest.mark.parametrize("d,dtype", [(64, HF), (128, BF)])
+@pytest.mark.parametrize("lens", [[(9, 1100)], [(64, 5000), (30, 700)], [(200, 3000)], [(130, 1024), (0, 3), (1, 2500)]])
+def test_many_queries_over_long_keys(lens, d, dtype):
+    """Few tiles over long keys: the key blocks are split and joined."""
+    run(lens, 4, 2, d, dtype, causal=True, spare=4)
+    run(lens, 4, 2, d, dtype, softcap=30.0, slopes=torch.rand(4, device="cuda"))
+    dq, dk = documents(lens, [100, 640, 1000])
+    run(lens, 4, 2, d, dtype, causal=True, doc_q=dq, doc_k=dk)
+    dq[::3] = 55  # see the prefix alone, or nothing
+    run(lens, 4, 2, d, dtype, doc_q=dq, doc_k=dk)
+    prefix = torch.full((len(lens),), 70, dtype=torch.int32, device="cuda")
+    bad = torch.zeros(len(dk), dtype=torch.bool, device="cuda")
+    at = torch.cat([torch.arange(b) for _, b in lens]).cuda()
+    dk[(at >= 70) & (at % 4 == 0)] = 77
+    bad[dk == 77] = True
+    run(lens, 4, 2, d, dtype, doc_q=dq, doc_k=dk, prefix=prefix,
+        poison=lambda q, k, v: (k.__setitem__(bad.nonzero().flatten(), math.nan), v.__setitem__(bad.nonzero().flatten(), math.inf)))
