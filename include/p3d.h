@@ -247,9 +247,10 @@ int p3d_linear_headnorm(p3d_ctx *ctx, const void *x, int64_t ldx, const void *w,
  * result does not depend on rounding on the way).  A row holding an infinity
  * or a NaN gets the scale NaN and zeros, so products with it are NaN.  x
  * [m][ldx] of dtype, q [m][ldq], scale f32 [m]; columns [0, k) of q are
- * written.  Any k and any leading dimensions >= k; rows on 16-byte boundaries
- * are written fastest.  Quantises activations by token and weights [n][k] by
- * output channel. */
+ * written.  Any k and any leading dimensions >= k; q and x must not overlap.
+ * Rows of x are read in whole 16-byte words (what lies beside them in a word is
+ * not used).  Quantises activations by token and weights [n][k] by output
+ * channel. */
 int p3d_quantize_rows(p3d_ctx *ctx, const void *x, int64_t ldx, int64_t m, int64_t k, int dtype, int8_t *q,
                       int64_t ldq, float *scale);
 
@@ -323,7 +324,7 @@ int p3d_varlen_attention(p3d_ctx *ctx, const void *q, int64_t ldq, const void *k
 
 /* Rules of p3d_masked_attention; zeros and NULLs mean none. */
 typedef struct p3d_attention_rules {
-    float softcap;         /* > 0: scores become softcap * tanh(score / softcap) */
+    float softcap;         /* 1e-6 .. 1e6: scores become softcap * tanh(score / softcap); 0: none */
     int causal;            /* nonzero: a query sees the keys up to its own position */
     const int32_t *prefix; /* [nseq]: the first prefix[s] keys of sequence s are seen by all its queries */
     const int32_t *doc_q;  /* [rows_q] and [rows_k], both or none: a query sees the keys of its own */

@@ -339,6 +339,7 @@ PyObject *masked_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     rules.slopes = vector<float>(a[14], heads, at::kFloat, dev, what, "slopes");
     const float scale = real(a[8]);
     const int64_t max_q = std::min(integer(a[5]), rows_q), max_k = std::min(integer(a[6]), rows_k);
+    need(max_q >= 0 && max_k >= 0, what, "max_q and max_k must not be negative");
     Tensor out, ws;
     int64_t ldo = width;
     if (a[16] == Py_None) {

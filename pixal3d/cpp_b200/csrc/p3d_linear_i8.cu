@@ -534,7 +534,7 @@ int launch_tiles(p3d_ctx *ctx, I8Params p) {
     int rc = make_tmap_i8(ctx, &ta, p.x, p.M, p.K, p.ldx, kTileM);
     if (rc || (rc = make_tmap_i8(ctx, &tb, p.w, p.N, p.K, p.ldw, BN))) return rc;
     const int64_t es = static_cast<int64_t>(dtype_size(p.out_dtype));
-    p.tma_out = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo * es % 16 == 0;
+    p.tma_out = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo * es % 16 == 0 && p.ldo >= p.N;
     if (p.tma_out && (rc = make_tmap_i8_out(ctx, &to, p))) return rc;
     p.wide_cols = ((reinterpret_cast<uintptr_t>(p.ws) | reinterpret_cast<uintptr_t>(p.bias)) & 15) == 0;
     P3D_CUDA(ctx, cudaFuncSetAttribute(linear_i8_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));

@@ -146,7 +146,8 @@ extern "C" int p3d_masked_attention(p3d_ctx *ctx, const void *q, int64_t ldq, co
                 "p3d_masked_attention: q/k/v/out must be 16-byte aligned");
     p3d_attention_rules r{};
     if (rules) r = *rules;
-    P3D_REQUIRE(ctx, r.softcap >= 0.0f && std::isfinite(r.softcap), "p3d_masked_attention: softcap must be finite, 0 for none");
+    P3D_REQUIRE(ctx, r.softcap == 0.0f || (r.softcap >= 1e-6f && r.softcap <= 1e6f),
+                "p3d_masked_attention: softcap must be 0 (none) or between 1e-6 and 1e6");
     P3D_REQUIRE(ctx, (r.doc_q == nullptr) == (r.doc_k == nullptr) || rows_k == 0,
                 "p3d_masked_attention: doc_q and doc_k go together");
     const size_t need = p3d_masked_attention_workspace(nseq, max_q, max_k, rows_q, rows_k, heads, kv_heads, head_dim,

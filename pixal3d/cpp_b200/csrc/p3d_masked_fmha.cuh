@@ -27,7 +27,7 @@
 //
 // Few CTAs over long keys: the visits are cut into splits, whose sums against
 // their own maxima a second kernel joins (one sequence of 64 queries, 16 heads
-// of 64, 8192 keys: SPLITOFF us without, SPLITON with).
+// of 64, 8192 keys: 106 us without, 21.7 with).
 //
 // Rows past the sequence's end compute on whatever the tile holds and are not
 // stored.  Every wait is bounded.
@@ -104,16 +104,13 @@ __device__ __forceinline__ bool clean_pair(uint32_t &w) {
     return lo || hi;
 }
 
-// Scores to capped scores in units of log2, c1 tanh(t) with t = s c0 / (2 log2
-// e).  While every t of the warp's rows is within 1/2 (scores within half the
-// cap) tanh(t) = t q(t^2), q of degree 3 fitted to an absolute error of 1.3e-7
-// (least maximum over [0, 1/2]), on the FMA pipe in pairs; otherwise by the
-// exponential and a reciprocal, which with the weights' own exponential are
-// three operations of the XU pipe for each score instead of one
-// (8192 x 8192, 16 heads of 128: XXX against YYY us).
+// Scores to capped scores, as capped(): by its polynomial on the FMA pipe in
+// pairs while every score of the warp's rows allows it, else by the exponential
+// and a reciprocal, which with the weights' own exponential are three operations
+// of the XU pipe for each score instead of one (8192 x 8192, 16 heads of 128:
+// 631 against 926 us).
 __device__ __forceinline__ void cap_row(float (&s)[64], float c0, float c1) {
-    constexpr float kHalfLn2 = 0.34657359027997264f;
-    const float ct = c0 * kHalfLn2;
+    const float ct = c0 * kCapT;
     float top = 0.0f;
 #pragma unroll
     for (int e = 0; e < 64; e += 4) {
@@ -122,7 +119,7 @@ __device__ __forceinline__ void cap_row(float (&s)[64], float c0, float c1) {
         top = max3f(max3f(top, fabsf(s[e]), fabsf(s[e + 1])), fabsf(s[e + 2]), fabsf(s[e + 3]));
     }
     if (__all_sync(0xffffffffu, top <= 0.5f)) {
-        const float k0 = 0.999997676f * c1, k1 = -0.333206552f * c1, k2 = 0.131451456f * c1, k3 = -0.043372481f * c1;
+        const float k0 = kCap0 * c1, k1 = kCap1 * c1, k2 = kCap2 * c1, k3 = kCap3 * c1;
 #pragma unroll
         for (int e = 0; e < 64; e += 2) {
             const F2 t(s[e], s[e + 1]);
@@ -132,7 +129,7 @@ __device__ __forceinline__ void cap_row(float (&s)[64], float c0, float c1) {
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < 64; ++e) s[e] = capped(s[e], 2.885390081777927f, c1);
+        for (int e = 0; e < 64; ++e) s[e] = capped_far(s[e], c1);
     }
 }
 

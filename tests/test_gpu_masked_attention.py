@@ -394,3 +394,44 @@ def test_many_queries_over_long_keys(lens, d, dtype):
     bad[dk == 77] = True
     run(lens, 4, 2, d, dtype, doc_q=dq, doc_k=dk, prefix=prefix,
         poison=lambda q, k, v: (k.__setitem__(bad.nonzero().flatten(), math.nan), v.__setitem__(bad.nonzero().flatten(), math.inf)))
+
+
+@pytest.mark.parametrize("d,dtype", [(64, HF), (128, BF)])
+@pytest.mark.parametrize("lens", [[(1, 300)], [(2, 900)], [(150, 200)]])
+def test_large_and_small_caps(lens, d, dtype):
+    """A cap far above the scores changes them by 2.4e-6 of themselves (and the
+    tanh by nothing): the uncapped result.  One far below them flattens them."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    nq, nk = lens[0]
+    q, k, v = (torch.randn((n, 2 * d), device="cuda", generator=g).to(dtype) for n in (nq, nk, nk))
+    q = q * 4
+    args = (cu([nq]), cu([nk]), nq, nk, 2, 1 / math.sqrt(d))
+    want, tol = attention64(q, k, v, lens, 2, 2, 1 / math.sqrt(d))
+    score = float((q.double().reshape(nq, 2, d).norm(dim=2).max() * k.double().reshape(nk, 2, d).norm(dim=2).max()) / math.sqrt(d))
+    for cap in (1e5, 1e6):
+        got = ops().masked_attention(q, k, v, *args, softcap=cap)
+        assert bool(((got.double() - want).abs() <= tol + 2 * 2.4e-6 * score * 2 * v.double().abs().amax()).all())
+    got = ops().masked_attention(q, k, v, *args, softcap=1e-6)
+    mean = v.double().mean(0)
+    u = torch.finfo(dtype).eps / 2
+    # every weight is 1 within 2e-6 and its rounding; the mean's own rounding; f32 sums
+    bound = (u * 1.01 + 4e-6 + nk * 2.0 ** -24) * 2 * v.double().abs().mean(0) + u * mean.abs() + 2.0 ** -24
+    assert bool(((got.double() - mean).abs() <= bound).all())
+
+
+def test_more_refusals():
+    from pixal3d.cpp_b200 import _lib as l
+    o = ops()
+    q = torch.zeros((4, 128), device="cuda").half()
+    c = cu([4])
+    for bad in (dict(softcap=1e7), dict(softcap=1e-9), dict(softcap=math.inf)):
+        with pytest.raises(l.P3DError) as e:
+            o.masked_attention(q, q, q, c, c, 4, 4, 2, 1.0, **bad)
+        assert e.value.status == l.P3D_ERR_INVALID
+    for bad in (lambda: o.masked_attention(q, q, q, c, c, -1, 4, 2, 1.0), lambda: o.masked_attention(q, q, q, c, c, 4, -1, 2, 1.0),
+                lambda: o.masked_attention(q, q, q, c, c, 4, 4, 0, 1.0), lambda: o.masked_attention(q, q[:, :64], q, c, c, 4, 4, 2, 1.0),
+                lambda: o.masked_attention(q, q.t().contiguous().t(), q, c, c, 4, 4, 2, 1.0)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(TypeError):
+        o.masked_attention(q, q, None, c, c, 4, 4, 2, 1.0)
