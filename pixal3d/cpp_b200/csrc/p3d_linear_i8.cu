@@ -583,11 +583,16 @@ extern "C" int p3d_linear_i8(p3d_ctx *ctx, const int8_t *x, int64_t ldx, const f
     // 6144 7.2 / 6.4.
     const int64_t kk = std::max<int64_t>(k, 512);
     if (m * n * kk < 18000000 + 34500 * kk) {
-        if (m == 1) return launch_rows<1, 1>(ctx, p);
-        // two channels a warp once that leaves every SM 16 warps
-        // (4 x 1024 x 6144: 3.3 against 4.6 us; 4 x 4096 x 1024: 6.5 / 4.3)
-        if (ceil_div(n, 2) * ceil_div(m, 4) >= 16 * 148) return launch_rows<4, 2>(ctx, p);
-        return launch_rows<2, 1>(ctx, p);
+        // Rows and channels a warp: as many as leave the GPU enough warps.  us
+        // with the choice and with 1 x 1 / 4 x 2: 1 x 1024 x 6144 2.16 (2.54 /
+        // 3.19), 2 x 1024 x 6144 2.33 (3.69 / 3.19), 2 x 4096 x 1024 3.04 (3.18
+        // / 3.98), 4 x 1024 x 6144 2.77 (6.87 / 3.20), 4 x 4096 x 1024 3.31
+        // (3.41 / 4.03), 16 x 4096 x 1024 4.69 (7.62 / the choice).
+        const bool wide = n >= 4096;
+        if (m == 2 && wide) return launch_rows<2, 4>(ctx, p);
+        if (m > 2 && m <= 4 && wide) return launch_rows<4, 4>(ctx, p);
+        if (m > 2 && ceil_div(n, 2) * ceil_div(m, 4) >= 1024) return launch_rows<4, 2>(ctx, p);
+        return launch_rows<1, 2>(ctx, p);
     }
     // The tile width of the fewest waves, a 128- and a 64-column tile costing
     // 0.78 and 0.69 of a 256-column one (8184 x 4096 x 1024: 11.4, 10.1 and
