@@ -576,13 +576,13 @@ extern "C" int p3d_linear_i8(p3d_ctx *ctx, const int8_t *x, int64_t ldx, const f
     DeviceGuard on(ctx->device);
     I8Params p{x, w, ldx, ldw, x_scale, w_scale, bias, out, ldo, gate, gate_ld, batch_offsets, nbatch,
                m, n, static_cast<int>(k), out_dtype, epilogue, ctx->fault, 0, 0};
-    // Few outputs: the rows kernel runs about 2 us + m n k / 15e6 us (k at
-    // least 512, a warp's stride), the tiles never under 3.2 us + 0.0023 us k
-    // (their ring of TMA loads).  m x k x n: 8 x 1024 x 6144 4.9 against 6.7 us,
-    // 16 x 4096 x 1024 7.2 / 12.7, 64 x 256 x 512 3.1 / 4.1, but 16 x 1024 x
-    // 6144 7.2 / 6.4.
+    // Few outputs: the rows kernel runs about 1.5 us + m n k / 21e6 us (16e6
+    // for short k; k at least 512, a warp's stride), the tiles 3.6 us + 0.0022
+    // us k (their ring of TMA loads).  m x k x n, rows against tiles: 120 x 333
+    // x 777 4.80 / 4.91 us, 200 x 100 x 600 5.74 / 4.08, 64 x 1024 x 1024 4.69 /
+    // 5.58, 16 x 1024 x 6144 6.24 / 6.74, 32 x 4096 x 1024 7.7 / 12.5.
     const int64_t kk = std::max<int64_t>(k, 512);
-    if (m * n * kk < 18000000 + 34500 * kk) {
+    if (m * n * kk < std::min<int64_t>(111000 * kk - 21000000, 47000 * kk + 45000000)) {
         // Rows and channels a warp: as many as leave the GPU enough warps.  us
         // with the choice and with 1 x 1 / 4 x 2: 1 x 1024 x 6144 2.16 (2.54 /
         // 3.19), 2 x 1024 x 6144 2.33 (3.69 / 3.19), 2 x 4096 x 1024 3.04 (3.18
