@@ -19,12 +19,17 @@ namespace {
 // this many keys, to the one that takes each query alone.
 constexpr int64_t kFewRows = 8, kFewKeys = 512;
 
+// Query tiles that are ordered at most: more of them leave a last wave too
+// short to matter.
+constexpr int kOrderTiles = 1024;
+
 size_t align256(size_t b) { return (b + 255) / 256 * 256; }
 
 // Smallest and largest document number of every key block, a warp a block.
 __global__ void __launch_bounds__(256) doc_range_kernel(const MaskedParams p) {
     pdl_wait();
     pdl_trigger();
+    if (p.tile_count && threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) *p.tile_count = 0;
     const SeqRange sr = seq_range(p, blockIdx.y);
     const int lane = threadIdx.x & 31, step = gridDim.x * 8;
     for (int b = blockIdx.x * 8 + (threadIdx.x >> 5); b * 64 < sr.lk; b += step) {
@@ -35,13 +40,76 @@ __global__ void __launch_bounds__(256) doc_range_kernel(const MaskedParams p) {
     }
 }
 
-// Many queries: the documents' block ranges, then the tensor-core kernel.
+// The order of the query tiles: those with the most key blocks first.  A tile
+// that holds the end of one document and the start of the next reads both, so
+// where it came late its CTA ran on alone (16384 queries in 5 documents, 16
+// heads: ORDER_OLD against ORDER_NEW us with this kernel's own time).  A warp
+// counts a tile's blocks as the attention kernel will visit them; the last
+// block ranks the counts.  Every tile comes once whatever the counts are, and
+// none depends on another: the order changes no result.
+__global__ void __launch_bounds__(256) doc_order_kernel(const MaskedParams p, int tiles) {
+    __shared__ int counts[kOrderTiles];
+    __shared__ int last;
+    pdl_wait();
+    pdl_trigger();
+    const int n = tiles * p.nseq, lane = threadIdx.x & 31, item = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (item < n) {
+        const int seq = item / tiles, row0 = item % tiles * 128;
+        const SeqRange sr = seq_range(p, seq);
+        const int nrows = min(min(sr.lq, static_cast<int>(p.max_q)) - row0, 128);
+        int count = -1, lo = 0x7fffffff, hi = -0x7fffffff - 1;
+        if (nrows > 0) {
+#pragma unroll
+            for (int r = 0; r < 128; r += 32) {
+                const int d = p.doc_q[sr.q0 + row0 + min(r + lane, nrows - 1)];
+                lo = min(lo, d);
+                hi = max(hi, d);
+            }
+            lo = __reduce_min_sync(0xffffffffu, lo);
+            hi = __reduce_max_sync(0xffffffffu, hi);
+            const int pre = p.prefix ? min(max(p.prefix[seq], 0), sr.lk) : 0;
+            const int limit = p.causal ? min(sr.lk, max(pre, row0 + nrows + sr.lk - sr.lq)) : sr.lk;
+            const int2 *range = p.doc_range + doc_block(sr, seq);
+            count = 0;
+#pragma unroll 4
+            for (int b = lane; b * 64 < limit; b += 32) {
+                const int2 r = range[b];
+                count += b * 64 < pre || (r.x <= hi && lo <= r.y);
+            }
+            count = __reduce_add_sync(0xffffffffu, count);
+        }
+        if (lane == 0) __stcg(p.tile_found + item, make_int4(count, lo, hi, item));
+    }
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(p.tile_count, 1) == static_cast<int>(gridDim.x) - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    for (int i = threadIdx.x; i < n; i += 256) counts[i] = __ldcg(&p.tile_found[i].x);
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int mine = counts[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += counts[j] > mine || (counts[j] == mine && j < i);
+        p.tile_order[rank] = __ldcg(p.tile_found + i);
+    }
+}
+
+// Many queries: the documents' block ranges and the tiles' order, then the
+// tensor-core kernel.
 int masked_attention_tiles(p3d_ctx *ctx, const MaskedParams &p, int head_dim, int dtype) {
     if (p.doc_k) {
         const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(ceil_div(std::max<int64_t>(p.max_k, 1), 8 * 64), 1024));
         P3D_CUDA(ctx, launch_pdl(doc_range_kernel, dim3(blocks, p.nseq), dim3(256), 0, ctx->stream, p));
-        const int rc = check_launch(ctx, "doc_range");
+        int rc = check_launch(ctx, "doc_range");
         if (rc) return rc;
+        if (p.tile_order) {
+            const int tiles = static_cast<int>(ceil_div(p.max_q, 128));
+            P3D_CUDA(ctx, launch_pdl(doc_order_kernel, dim3(static_cast<unsigned>(ceil_div(tiles * p.nseq, 8))), dim3(256), 0, ctx->stream,
+                                     p, tiles));
+            if ((rc = check_launch(ctx, "doc_order"))) return rc;
+        }
     }
     if (dtype == P3D_BF16) return head_dim == 64 ? masked_tiles_bf16_64(ctx, p, dtype) : masked_tiles_bf16_128(ctx, p, dtype);
     return head_dim == 64 ? masked_tiles_f16_64(ctx, p, dtype) : masked_tiles_f16_128(ctx, p, dtype);
@@ -84,14 +152,20 @@ struct PiecePlan {
 };
 
 // Many queries: splits of the key blocks (where the CTAs would fill less than
-// half of the GPU's 296 places, pieces of at least 8 blocks) and the bytes of
-// the documents' ranges and of the splits' results.
+// half of the GPU's 296 places, pieces of at least 8 blocks), whether the tiles
+// are ordered (documents, more CTAs than places), and the bytes of the
+// documents' ranges, of the order and of the splits' results.
 struct TilePlan {
     int splits;
-    size_t docs, o, ml;
+    int64_t tiles;
+    bool ordered;
+    size_t docs, order, o, ml;
     TilePlan(int nseq, int64_t max_q, int64_t max_k, int64_t rows_q, int64_t rows_k, int heads, int head_dim, bool documents) {
         const int64_t ctas = static_cast<int64_t>(heads) * nseq * ceil_div(max_q, 128);
         splits = ctas > 148 ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({296 / std::max<int64_t>(ctas, 1), max_k / 512, 16})));
+        tiles = nseq * ceil_div(max_q, 128);
+        ordered = documents && ctas > 296 && tiles <= kOrderTiles;
+        order = ordered ? align256(static_cast<size_t>(2 * tiles + 1) * sizeof(int4)) : 0;
         docs = documents ? align256(static_cast<size_t>(rows_k / 64 + nseq + 1) * sizeof(int2)) : 0;
         const size_t parts = splits > 1 ? static_cast<size_t>(rows_q) * heads * splits : 0;
         o = align256(parts * head_dim * sizeof(float));
@@ -109,7 +183,7 @@ extern "C" size_t p3d_masked_attention_workspace(int nseq, int64_t max_q, int64_
     if (nseq <= 0 || max_q <= 0 || max_k < 0 || rows_q <= 0 || rows_k < 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
     if (max_q > kFewRows) {
         const TilePlan plan(nseq, max_q, max_k, rows_q, rows_k, heads, head_dim, documents != 0);
-        return plan.docs + plan.o + plan.ml;
+        return plan.docs + plan.order + plan.o + plan.ml;
     }
     if (max_k <= kFewKeys) return 0;
     const PiecePlan plan(nseq, max_q, max_k, rows_k, heads, kv_heads, head_dim);
@@ -188,8 +262,15 @@ extern "C" int p3d_masked_attention(p3d_ctx *ctx, const void *q, int64_t ldq, co
         char *at = static_cast<char *>(ws);
         p.splits = plan.splits;
         p.doc_range = reinterpret_cast<int2 *>(at);
-        p.part_o = reinterpret_cast<float *>(at + plan.docs);
-        p.part_ml = reinterpret_cast<float2 *>(at + plan.docs + plan.o);
+        at += plan.docs;
+        if (plan.ordered) {
+            p.tile_found = reinterpret_cast<int4 *>(at);
+            p.tile_order = p.tile_found + plan.tiles;
+            p.tile_count = reinterpret_cast<int *>(p.tile_order + plan.tiles);
+        }
+        at += plan.order;
+        p.part_o = reinterpret_cast<float *>(at);
+        p.part_ml = reinterpret_cast<float2 *>(at + plan.o);
         return masked_attention_tiles(ctx, p, head_dim, dtype);
     }
     if (max_k <= kFewKeys) return masked_attention_rows(ctx, p, head_dim, dtype);

@@ -28,6 +28,11 @@ struct MaskedParams {
     float *part_o;
     float2 *part_ml;
     int2 *doc_range; // (smallest, largest) document number of every 64-key block
+    // many queries of documents: (key blocks, smallest and largest document
+    // number, sequence * tiles + tile) of the query tiles as they lie, and by
+    // their blocks, largest first (null: not ordered); a counter
+    int4 *tile_found, *tile_order;
+    int *tile_count;
     int *fault;
 };
 

@@ -159,9 +159,19 @@ __global__ void __launch_bounds__(kThreadsF, 2)
     using C = Cfg<D>;
     constexpr int ST = C::STAGES;
     pdl_wait();
-    const int head = blockIdx.x, seq = blockIdx.y;
-    const int split = blockIdx.z % p.splits, z = blockIdx.z / p.splits;
-    const int tile = p.causal ? gridDim.z / p.splits - 1 - z : z;  // the longest rows first
+    const int head = blockIdx.x;
+    int seq = blockIdx.y;
+    const int split = blockIdx.z % p.splits, z = blockIdx.z / p.splits, tiles = gridDim.z / p.splits;
+    int tile = p.causal ? tiles - 1 - z : z;  // the longest rows first
+    int qdoc_lo = 0, qdoc_hi = 0;  // documents of the tile's queries
+    const bool ordered = DOCS && p.tile_order;
+    if (ordered) {
+        const int4 item = p.tile_order[z * p.nseq + seq];
+        seq = item.w / tiles;
+        tile = item.w % tiles;
+        qdoc_lo = item.y;
+        qdoc_hi = item.z;
+    }
     const SeqRange sr = seq_range(p, seq);
     const int row0 = tile * kM;                       // first query of the tile, within the sequence
     const int nrows = min(min(sr.lq, static_cast<int>(p.max_q)) - row0, kM);
@@ -216,7 +226,6 @@ __global__ void __launch_bounds__(kThreadsF, 2)
     const int pos_lo = row0 + shift, pos_hi = row0 + nrows - 1 + shift;
     const int limit = p.causal ? min(sr.lk, max(pre, pos_hi + 1)) : sr.lk;  // no query of the tile sees a key from here on
     const int blocks = max(0, (limit + kN - 1) / kN);
-    int qdoc_lo = 0, qdoc_hi = 0;
     // this split's share of the visits
     int chunk = static_cast<int>(static_cast<int64_t>(blocks) * split / p.splits);
     const int visits = static_cast<int>(static_cast<int64_t>(blocks) * (split + 1) / p.splits);
@@ -257,7 +266,7 @@ __global__ void __launch_bounds__(kThreadsF, 2)
     bool cur_mixed = false;
     int cur = -1;
     if (warp == 0) {
-        if (DOCS) {
+        if (DOCS && !ordered) {
             int lo = 0x7fffffff, hi = -0x7fffffff - 1;
             for (int r = lane; r < nrows; r += 32) {
                 const int d = p.doc_q[sr.q0 + row0 + r];

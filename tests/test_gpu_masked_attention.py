@@ -435,3 +435,60 @@ def test_more_refusals():
             bad()
     with pytest.raises(TypeError):
         o.masked_attention(q, q, None, c, c, 4, 4, 2, 1.0)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("d,dtype", [(64, HF), (128, BF)])
+@pytest.mark.parametrize("lens", [[(1100, 1100), (0, 40), (300, 700), (9, 0)], [(9, 30)] * 31])
+def test_documents_of_more_tiles_than_places(lens, d, dtype, causal):
+    """Tiles are taken in the order of their key blocks: sorted documents, numbers in any order, empty tiles and sequences."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    dq, dk = documents(lens, [3, 70, 500, 620, 1000])
+    prefix = torch.arange(len(lens), dtype=torch.int32, device="cuda") * 7 - 5
+    run(lens, 10, 5, d, dtype, causal=causal, doc_q=dq, doc_k=dk, prefix=prefix)
+    dq, dk = (torch.randint(-3, 5, x.shape, device="cuda", generator=g).int() for x in (dq, dk))
+    got = run(lens, 12, 1, d, dtype, causal=causal, doc_q=dq, doc_k=dk)
+    assert torch.equal(got, run(lens, 12, 1, d, dtype, causal=causal, doc_q=dq, doc_k=dk))
+
+
+@pytest.mark.parametrize("sequences", [1024, 1025])
+def test_documents_of_many_sequences(sequences):
+    """The most tiles that are ordered, and one more."""
+    lens = [(9 + i % 3, 11 + i % 70) for i in range(sequences)]
+    dq, dk = documents(lens, [5, 40, 64])
+    run(lens, 1, 1, 64, HF, doc_q=dq, doc_k=dk)
+
+
+def test_ordered_documents_in_graphs_and_on_streams():
+    """One workspace, two captured calls replayed in turn and a call on another stream: each call counts its tiles anew."""
+    o = ops()
+    n, heads, d = 1500, 30, 64
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q, k, v = (torch.randn((n, heads * d), device="cuda", generator=g).half() for _ in range(3))
+    doc = torch.bucketize(torch.arange(n), torch.tensor([100, 900, 1000]), right=True).int().cuda()
+
+    def call(doc):
+        return o.masked_attention(q, k, v, cu([n]), cu([n]), n, n, heads, 0.125, doc_q=doc, doc_k=doc)
+
+    other = doc.flip(0).contiguous()
+    want = call(doc), call(other)
+    c = cu([n])
+    graphs = []
+    for x in (doc, other):
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = o.masked_attention(q, k, v, c, c, n, n, heads, 0.125, doc_q=x, doc_k=x)
+        graphs.append((gr, out))
+    for _ in range(3):
+        for (gr, out), w in zip(graphs, want):
+            out.fill_(1.0)
+            gr.replay()
+            assert torch.equal(out, w)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = call(other)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want[1])
+    o.ctx().sync_check()
