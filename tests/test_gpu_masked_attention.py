@@ -492,3 +492,23 @@ def test_ordered_documents_in_graphs_and_on_streams():
     torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(got, want[1])
     o.ctx().sync_check()
+
+
+@pytest.mark.parametrize("d,dtype", [(64, HF), (128, BF)])
+def test_documents_that_come_late(d, dtype):
+    """Inputs far from the SMs: loads of masks end before or after those of keys, and no wait runs out."""
+    o = ops()
+    g = torch.Generator(device="cuda").manual_seed(9)
+    n, heads = 1300, 30
+    q, k, v = (torch.randn((n, heads * d), device="cuda", generator=g).to(dtype) for _ in range(3))
+    doc = torch.bucketize(torch.arange(n), torch.tensor([64, 200, 210, 700]), right=True).int().cuda()
+    slopes = torch.rand(heads, device="cuda", generator=g)
+    flush = torch.empty(64 << 20, dtype=torch.int32, device="cuda")
+    c = cu([n])
+    want = o.masked_attention(q, k, v, c, c, n, n, heads, 0.1, doc_q=doc, doc_k=doc, slopes=slopes)
+    o.ctx().sync_check()
+    for i in range(40):
+        flush.fill_(i)
+        got = o.masked_attention(q, k, v, c, c, n, n, heads, 0.1, doc_q=doc, doc_k=doc, slopes=slopes)
+        o.ctx().sync_check()
+        assert torch.equal(got, want)
