@@ -89,12 +89,29 @@ __device__ __forceinline__ float max3f(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
+__device__ __forceinline__ float min3f(float a, float b, float c) {
+    float r;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ float row_max64(const float (&s)[64]) {
     float m[8];
 #pragma unroll
     for (int c = 0; c < 8; ++c)
         m[c] = fmaxf(max3f(max3f(max3f(s[c], s[8 + c], s[16 + c]), s[24 + c], s[32 + c]), s[40 + c], s[48 + c]), s[56 + c]);
     return max3f(max3f(m[0], m[1], m[2]), max3f(m[3], m[4], m[5]), fmaxf(m[6], m[7]));
+}
+
+__device__ __forceinline__ float row_min64(const float (&s)[64]) {
+    float m[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        m[c] = s[c];
+#pragma unroll
+        for (int e = 4 + c; e < 60; e += 8) m[c] = min3f(m[c], s[e], s[e + 4]);
+        m[c] = fminf(m[c], s[60 + c]);
+    }
+    return fminf(min3f(m[0], m[1], m[2]), m[3]);
 }
 
 // Infinities and NaN of a packed pair set to zero.
@@ -146,6 +163,22 @@ __device__ __forceinline__ void cap_row(float (&s)[64], float c0, float c1) {
         for (int e = 0; e < 64; ++e) s[e] = capped_far(s[e], c1);
     }
 }
+
+// The polynomial of near capped scores with its factors folded in: the capped
+// score in units of log2 is s (f0 + u (f1 + u (f2 + u f3))), u = s^2, for
+// |s| <= top; top < 0 where a factor would leave 32 bits' range.
+struct NearCap {
+    float f0, f1, f2, f3, top;
+    __device__ __forceinline__ NearCap(float c0, float c1) {
+        const float ct = c0 * kCapT, cc = ct * ct;
+        f0 = kCap0 * c1 * ct;
+        f1 = kCap1 * c1 * ct * cc;
+        f2 = kCap2 * c1 * ct * cc * cc;
+        f3 = kCap3 * c1 * ct * cc * cc * cc;
+        const bool fits = fabsf(f0) > 1e-30f && fabsf(f0) < 1e30f && fabsf(f3) > 1e-30f && fabsf(f3) < 1e30f;
+        top = fits ? 0.5f / ct : -1.0f;
+    }
+};
 
 // s scale - slope |d - e| for the 64 keys e of a block, d the query's position
 // relative to the block's first key.  A block that lies on one side of all of
@@ -417,6 +450,7 @@ __global__ void __launch_bounds__(kThreadsF, 2)
         auto visible = [&](int j) -> bool {
             return j < edge && (j < pre || !DOCS || ((!p.causal || j <= pos) && p.doc_k[sr.k0 + j] == docq));
         };
+        const NearCap near(p.c0, p.c1);
         float m_run = -INFINITY;
         F2 l2(0.0f, 0.0f);
         bool ok = true;
@@ -470,7 +504,26 @@ __global__ void __launch_bounds__(kThreadsF, 2)
                         s[32 + e] = v1[e];
                     }
                 }
-                if constexpr (CAP) cap_row(s, p.c0, p.c1);
+                // Near capped scores of a block that the mask leaves whole: the cap
+                // rises with the score, so the maximum comes before it, and its last
+                // product takes the subtraction in (5 operations a pair, not 7; 2 x 4092
+                // queries, 16 heads of 64: 312 against 278 us; 8192, 16 of 128: 640
+                // against 618; 8192 in 3 documents, 16 of 128: 302 against 290; where
+                // documents are short and causal the spills of the two forms cost
+                // more than it gives: 8000 in 7, 32 of 128, 210 against 221).
+                bool folded = false;
+                float mx = 0.0f;
+                if constexpr (CAP && !BIAS) {
+                    if (all) {
+                        mx = row_max64(s);
+                        folded = __all_sync(0xffffffffu, fmaxf(mx, -row_min64(s)) <= near.top);
+                        const float u = mx * mx;
+                        mx *= fmaf(fmaf(fmaf(u, near.f3, near.f2), u, near.f1), u, near.f0);
+                    }
+                }
+                if constexpr (CAP) {
+                    if (!folded) cap_row(s, p.c0, p.c1);
+                }
                 if constexpr (BIAS) bias_row(s, CAP ? 1.0f : p.c0, slope, pos - j0);
                 if (!all) {
                     const int shared = pre - j0, own = (p.causal ? min(sr.lk, pos + 1) : sr.lk) - j0;
@@ -496,7 +549,7 @@ __global__ void __launch_bounds__(kThreadsF, 2)
                     }
                 }
                 const float unit = (CAP || BIAS) ? 1.0f : p.c0;
-                const float mx = row_max64(s) * unit;
+                if (!folded) mx = row_max64(s) * unit;
                 const bool need = i > 0 && mx > m_run + kRescaleLog2;
                 if (i == 0) m_run = mx;
                 if (__any_sync(0xffffffffu, need)) {
@@ -519,14 +572,25 @@ __global__ void __launch_bounds__(kThreadsF, 2)
                 }
                 // a row that has seen no key yet has nothing to subtract: its weights are 2^-inf
                 const float nm = m_run == -INFINITY ? 0.0f : -m_run;
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
+                auto weights = [&](int e, F2 x) {
                     float x0, x1;
-                    fma2(F2(s[2 * e], s[2 * e + 1]), F2(unit, unit), F2(nm, nm)).get(x0, x1);
+                    x.get(x0, x1);
                     x0 = ex2f(x0);
                     x1 = ex2f(x1);
                     l2 = add2(l2, F2(x0, x1));
                     pk[e] = pack2<T>(x0, x1);
+                };
+                if (CAP && !BIAS && folded) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const F2 x(s[2 * e], s[2 * e + 1]), u = mul2(x, x);
+                        const F2 q = fma2(fma2(fma2(u, F2(near.f3, near.f3), F2(near.f2, near.f2)), u, F2(near.f1, near.f1)), u,
+                                          F2(near.f0, near.f0));
+                        weights(e, fma2(x, q, F2(nm, nm)));
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) weights(e, fma2(F2(s[2 * e], s[2 * e + 1]), F2(unit, unit), F2(nm, nm)));
                 }
             } else {
 #pragma unroll

@@ -512,3 +512,11 @@ def test_documents_that_come_late(d, dtype):
         got = o.masked_attention(q, k, v, c, c, n, n, heads, 0.1, doc_q=doc, doc_k=doc, slopes=slopes)
         o.ctx().sync_check()
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("d,dtype", [(64, HF), (64, BF), (128, HF), (128, BF)])
+def test_caps_near_and_far_from_the_scores(d, dtype, causal):
+    """Blocks whose scores all lie within half the cap, blocks with a row beyond it, and the largest score on either side of it."""
+    for softcap, sharp in ((50.0, 1.0), (50.0, 6.0), (8.0, 1.0), (3.0, 0.3), (1000.0, 4.0)):
+        run([(300, 300), (140, 500)], 4, 2, d, dtype, softcap=softcap, sharp=sharp, causal=causal)
