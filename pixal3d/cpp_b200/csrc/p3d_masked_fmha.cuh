@@ -135,11 +135,14 @@ __device__ __forceinline__ bool any_nonfinite(const uint4 &u) {
     return ((zero_half(u.x) | zero_half(u.y) | zero_half(u.z) | zero_half(u.w)) & 0x80008000u) != 0;
 }
 
-// Scores to capped scores, as capped(): by its polynomial on the FMA pipe in
-// pairs while every score of the warp's rows allows it, else by the exponential
-// and a reciprocal, which with the weights' own exponential are three operations
-// of the XU pipe for each score instead of one (8192 x 8192, 16 heads of 128:
-// 631 against 926 us).
+// Scores to capped scores, as capped(): each by its polynomial or, beyond half
+// the cap, by the exponential and a reciprocal, which with the weights' own
+// exponential are three operations of the XU pipe for each score instead of one
+// (8192 x 8192, 16 heads of 128: 584 us, 1145 with far scores in every block;
+// that form for all scores of such a block 1074).  Where no score of the
+// warp's rows is far the second form is left out; where one is, the others still
+// take the polynomial, whose error goes with the score and not with the cap
+// (the far one may be another row's, or a hidden key's).
 __device__ __forceinline__ void cap_row(float (&s)[64], float c0, float c1) {
     const float ct = c0 * kCapT;
     float top = 0.0f;
@@ -149,8 +152,8 @@ __device__ __forceinline__ void cap_row(float (&s)[64], float c0, float c1) {
         mul2(F2(s[e + 2], s[e + 3]), F2(ct, ct)).get(s[e + 2], s[e + 3]);
         top = max3f(max3f(top, fabsf(s[e]), fabsf(s[e + 1])), fabsf(s[e + 2]), fabsf(s[e + 3]));
     }
+    const float k0 = kCap0 * c1, k1 = kCap1 * c1, k2 = kCap2 * c1, k3 = kCap3 * c1;
     if (__all_sync(0xffffffffu, top <= 0.5f)) {
-        const float k0 = kCap0 * c1, k1 = kCap1 * c1, k2 = kCap2 * c1, k3 = kCap3 * c1;
 #pragma unroll
         for (int e = 0; e < 64; e += 2) {
             const F2 t(s[e], s[e + 1]);
@@ -160,7 +163,13 @@ __device__ __forceinline__ void cap_row(float (&s)[64], float c0, float c1) {
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < 64; ++e) s[e] = capped_far(s[e], c1);
+        for (int e = 0; e < 64; ++e) {
+            float t = s[e];
+            asm volatile("" : "+f"(t));  // in order: no more registers than the near form
+            const float u = t * t, f = capped_far(t, c1);
+            const float x = t * fmaf(fmaf(fmaf(u, k3, k2), u, k1), u, k0);
+            s[e] = fabsf(t) <= 0.5f ? x : f;
+        }
     }
 }
 

@@ -1,0 +1,67 @@
+"""Masked attention where roundings on the way could show."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tests.test_gpu_masked_attention import BF, HF, attention64, cu, documents, ops
+
+pytestmark = pytest.mark.gpu
+
+
+def capped(lens, d, dtype, cap, doc_q=None, doc_k=None, causal=False, poison=None, rows=None):
+    """A cap far above all scores but those of query rows `rows`: near scores
+    are at most 2.4e-6 of themselves off whatever lies beside them, so nothing
+    in the tolerance grows with the cap (the tanh itself takes s^3 / (3 cap^2),
+    below 1e-6 here)."""
+    o = ops()
+    g = torch.Generator(device="cuda").manual_seed(7)
+    nq, nk = sum(a for a, _ in lens), sum(b for _, b in lens)
+    q = torch.randn((nq + 9, 2 * d), device="cuda", generator=g).to(dtype)
+    k, v = (torch.randn((nk + 9, 2 * d), device="cuda", generator=g).to(dtype) for _ in range(2))
+    scale = 1 / math.sqrt(d)
+    rules = dict(causal=causal, doc_q=doc_q, doc_k=doc_k)
+    want, tol = attention64(q, k, v, lens, 2, 2, scale, **rules)
+    score = float(q[:nq].double().reshape(nq, 2, d).norm(dim=2).max() * k[:nk].double().reshape(nk, 2, d).norm(dim=2).max()) * scale
+    tol = tol + 2 * (2.4e-6 * score + 1e-6) * 2 * v[:nk].double().abs().amax()
+    if poison is not None:
+        poison(q, k, v)
+    got = o.masked_attention(q, k, v, cu([a for a, _ in lens]), cu([b for _, b in lens]), max(a for a, _ in lens), max(b for _, b in lens),
+                             2, scale, softcap=cap, **rules)
+    o.ctx().sync_check()
+    keep = torch.ones(nq, dtype=torch.bool, device="cuda")
+    if rows is not None:
+        keep[rows] = False
+    err = (got.double() - want).abs()[:nq][keep]
+    assert bool((err <= tol[:nq][keep]).all()), float((err / tol[:nq][keep]).max())
+
+
+CAPPED = [(64, HF), (64, BF), (128, HF), (128, BF)]
+
+
+@pytest.mark.parametrize("cap", [1e5, 1e6])
+@pytest.mark.parametrize("d,dtype", CAPPED)
+@pytest.mark.parametrize("lens", [[(200, 200), (90, 130)], [(30, 1500)], [(3, 700)], [(2, 100)]])
+def test_hidden_keys_leave_capped_scores_alone(lens, d, dtype, cap):
+    """One infinite element in hidden keys, and in rows behind the last sequence."""
+    dq, dk = documents(lens, [10 ** 6])
+    dk[5::9] = 99
+    dq, dk = torch.cat([dq, dq.new_full((9,), 7)]), torch.cat([dk, dk.new_full((9,), 7)])
+
+    def poison(q, k, v):
+        hidden = (dk == 99).nonzero().flatten()
+        k[hidden, 3] = k[hidden, d + 3] = math.inf
+        for t in (q, k, v):
+            t[-9:] = 3e4
+    capped(lens, d, dtype, cap, doc_q=dq, doc_k=dk, poison=poison)
+
+
+@pytest.mark.parametrize("cap", [3e4, 1e5])
+@pytest.mark.parametrize("d,dtype", CAPPED)
+@pytest.mark.parametrize("lens,row", [([(200, 200), (90, 130)], 37), ([(130, 400)], 129), ([(5, 700)], 2)])
+def test_far_scores_of_one_query_leave_the_others_alone(lens, row, d, dtype, cap):
+    """A query whose scores reach the cap beside queries whose scores do not."""
+    def poison(q, k, v):
+        q[row] = 6e4 * torch.sign(q[row].float()).to(dtype)
+    capped(lens, d, dtype, cap, poison=poison, rows=[row])
