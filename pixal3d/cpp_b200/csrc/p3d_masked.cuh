@@ -67,6 +67,18 @@ __device__ __forceinline__ float rcpf(float x) {
     return r;
 }
 
+// Weights are rounded to the operand type, since they are the second product's
+// operand: half a step (2^-8 of a bf16 weight, 2^-11 of an f16 one) of each
+// weight by itself.  f16 has few exponents, so there the running maximum is
+// held this many powers of two below the scores' own: weights down to 2^-29 of the
+// largest keep all their bits (2^-14 without) and those down to 2^-40 count
+// (2^-25).  Where the maximum may lag 8 behind, it is held 7 below instead of 15:
+// 2^-21 and 2^-32.  No weight passes 2^15.
+template <typename T>
+constexpr float kLift = 0.0f;
+template <>
+inline constexpr float kLift<__half> = 15.0f;
+
 // The capped score in units of log2, c1 tanh(t) with t = s c0 / (2 log2 e).
 // Scores within half the cap: t q(t^2), q of degree 3 fitted to an absolute
 // error of 1.3e-7 (least maximum over [0, 1/2]), 2.4e-6 of the score itself.

@@ -15,8 +15,9 @@
 // their row, apply the score rules (and, in mixed blocks only, the mask), and
 // write P_b over S_b as 16-bit; O += P_b V with P from TMEM.  The running
 // maximum is raised lazily: O and the sum are rescaled when a block's maximum
-// exceeds it by more than 8 (2^8 in P), which keeps P within 16-bit range and
-// the result exact, as both are taken against the same maximum.
+// exceeds it by more than 8 (2^8 in P; f16: 2^15, as the maximum is held lower),
+// which keeps P within 16-bit range and the result exact, as both are taken
+// against the same maximum.
 //
 // Hidden places: a hidden score is replaced by -inf whatever it was, but a
 // hidden key's V still meets P = 0 in the product, and 0 * NaN is NaN.  So the
@@ -559,6 +560,7 @@ __global__ void __launch_bounds__(kThreadsF, 2)
                 }
                 const float unit = (CAP || BIAS) ? 1.0f : p.c0;
                 if (!folded) mx = row_max64(s) * unit;
+                if constexpr (kLift<T> > 0.0f) mx -= kLift<T> - kRescaleLog2;
                 const bool need = i > 0 && mx > m_run + kRescaleLog2;
                 if (i == 0) m_run = mx;
                 if (__any_sync(0xffffffffu, need)) {

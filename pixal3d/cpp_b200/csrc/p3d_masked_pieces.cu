@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             mx[r] = fmaxf(mx[r], x);
                         }
                     mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2)) - kLift<T>;
                     raised |= mx[r] > m[r];
                 }
                 if (__any_sync(0xffffffffu, raised)) {

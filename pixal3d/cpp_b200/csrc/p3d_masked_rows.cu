@@ -140,7 +140,7 @@ __device__ __forceinline__ void rows_item(const MaskedParams &p, RowsShared<D, H
                     mx[r] = fmaxf(mx[r], x);
                 }
             mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2)) - kLift<T>;
             raised |= mx[r] > m[r];
         }
         if (__any_sync(0xffffffffu, raised)) {

@@ -65,3 +65,31 @@ def test_far_scores_of_one_query_leave_the_others_alone(lens, row, d, dtype, cap
     def poison(q, k, v):
         q[row] = 6e4 * torch.sign(q[row].float()).to(dtype)
     capped(lens, d, dtype, cap, poison=poison, rows=[row])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lq,n", [(1, 400), (7, 3000), (40, 3000), (1000, 900)])
+def test_f16_weights_far_below_the_largest(lq, n, d):
+    """Every sixteenth key has the largest weight and no value, the others 2^-18
+    to 2^-24 of it and large values.  Weights are rounded to f16 with the
+    largest at 2^7 or above: half a step of the smallest is 2^-32 of it."""
+    o = ops()
+    g = torch.Generator(device="cuda").manual_seed(d)
+    q, k, v = (torch.zeros((m, 2 * d), device="cuda") for m in (lq, n, n))
+    t = torch.linspace(12.5, 16.5, 2 * lq, device="cuda").reshape(lq, 2).half()
+    q[:, 0], q[:, d] = t[:, 0], t[:, 1]
+    k[:, 0] = k[:, d] = -1
+    v[:] = 500 + 1000 * torch.rand((1, 2 * d), device="cuda", generator=g)
+    k[5::16] = v[5::16] = 0
+    q, k, v = q.half(), k.half(), v.half()
+    got = o.masked_attention(q, k, v, cu([lq]), cu([n]), lq, n, 2, 1.0)
+    o.ctx().sync_check()
+    top = len(range(5, n, 16))
+    e = torch.exp(-t.double())[:, :, None]
+    want = e * (n - top) / (top + e * (n - top)) * v[0].double().reshape(2, d)
+    # a weight: half its step (2^-11 of it, or 2^-32 of the largest) and the exponential's 2^-19; it counts once in
+    # the mean and once in the sum; f32 sums of n terms; the result's own half step
+    rel = 2 * (2.0 ** -11 + 2.0 ** -32 / e + 2.0 ** -19 + n * 2.0 ** -24)
+    tol = want * (rel + 2.0 ** -11) * 1.01 + 2.0 ** -25
+    err = (got.double().reshape(lq, 2, d) - want).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
