@@ -33,7 +33,7 @@
 // the CTA still frees its TMEM and exits.
 #include <type_traits>
 
-#include "p3d_common.cuh"
+#include "p3d_fmha.cuh"
 
 namespace p3d {
 namespace {
@@ -64,41 +64,6 @@ static_assert(L_COL == O_COL + kD, "the row sum is accumulator column 64 of the 
 
 __device__ __forceinline__ uint32_t sp_col(int b) { return b ? 64u : 0u; }
 
-// D(tmem) (+)= A(tmem) * B(smem desc)^T, kind::f16.
-__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
-                                            uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
-        "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
-        "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// One TMEM column for the warp's 32 lanes.
-__device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
-    uint32_t r;
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr) : "memory");
-    return __uint_as_float(r);
-}
-__device__ __forceinline__ void tmem_st1(uint32_t taddr, float v) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(__float_as_uint(v))
-                 : "memory");
-}
-
 // 2^x0, 2^x1 as a packed 16-bit pair (x0 in the low half): one MUFU op.
 template <typename T>
 __device__ __forceinline__ uint32_t ex2_pair(float x0, float x1);
@@ -127,25 +92,6 @@ __device__ __forceinline__ void ffma2(float a0, float a1, float s, float c, floa
     asm("mov.b64 %0, {%1, %1};" : "=l"(cc) : "f"(c));
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(sc), "l"(cc));
     asm("mov.b64 {%0, %1}, %2;" : "=f"(d0), "=f"(d1) : "l"(d));
-}
-
-__device__ __forceinline__ float max3f(float a, float b, float c) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-
-// Row max of 64 scores: 8 chains of 3-input max, then a 3-input tree.
-__device__ __forceinline__ float row_max64(const float *s) {
-    float m[8];
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-        const float a = max3f(s[c], s[8 + c], s[16 + c]);
-        const float b = max3f(a, s[24 + c], s[32 + c]);
-        const float d = max3f(b, s[40 + c], s[48 + c]);
-        m[c] = fmaxf(d, s[56 + c]);
-    }
-    return max3f(max3f(m[0], m[1], m[2]), max3f(m[3], m[4], m[5]), fmaxf(m[6], m[7]));
 }
 
 // P for 64 scores: x = s * scale_log2 - m by packed f32x2 FMAs, 2^x in

@@ -37,6 +37,7 @@
 // stored.  Every wait is bounded.
 #include <type_traits>
 
+#include "p3d_fmha.cuh"
 #include "p3d_masked.cuh"
 
 namespace p3d {
@@ -62,47 +63,11 @@ struct Cfg {
     static_assert(STAGES + 2 <= kTags, "tag ring");
 };
 
-// D(tmem) (+)= A(tmem) * B(smem desc)^T, kind::f16.
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
-        "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
-        "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-__device__ __forceinline__ float max3f(float a, float b, float c) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
 __device__ __forceinline__ float min3f(float a, float b, float c) {
     float r;
     asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-__device__ __forceinline__ float row_max64(const float (&s)[64]) {
-    float m[8];
-#pragma unroll
-    for (int c = 0; c < 8; ++c)
-        m[c] = fmaxf(max3f(max3f(max3f(s[c], s[8 + c], s[16 + c]), s[24 + c], s[32 + c]), s[40 + c], s[48 + c]), s[56 + c]);
-    return max3f(max3f(m[0], m[1], m[2]), max3f(m[3], m[4], m[5]), fmaxf(m[6], m[7]));
-}
-
 __device__ __forceinline__ float row_min64(const float (&s)[64]) {
     float m[4];
 #pragma unroll
@@ -418,7 +383,7 @@ __global__ void __launch_bounds__(kThreadsF, 2)
                 const uint32_t v_addr = smem_u32(sV + st * C::KV_BYTES);
 #pragma unroll
                 for (int kk = 0; kk < kN / 16; ++kk)  // 16 keys: 8 packed TMEM columns of P, 2048 bytes of V
-                    umma_ts(tmem + kOCol, tmem + b * kN + kk * 8, sw128_desc_mn(v_addr + kk * 2048, kSub), idesc_o,
+                    umma_f16_ts(tmem + kOCol, tmem + b * kN + kk * 8, sw128_desc_mn(v_addr + kk * 2048, kSub), idesc_o,
                             (i > 0 || kk > 0) ? 1u : 0u);
                 umma_commit(&pv_done[b]);
                 umma_commit(&v_empty[st]);
