@@ -36,6 +36,8 @@ __device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr) : "memory");
     return __uint_as_float(r);
 }
+// tcgen05.wait::ld that holds back every use of v.
+__device__ __forceinline__ void tmem_ld_wait_reg(float &v) { asm volatile("tcgen05.wait::ld.sync.aligned;" : "+f"(v)::"memory"); }
 __device__ __forceinline__ void tmem_st1(uint32_t taddr, float v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(__float_as_uint(v))
                  : "memory");

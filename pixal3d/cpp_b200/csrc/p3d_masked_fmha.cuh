@@ -17,7 +17,12 @@
 // maximum is raised lazily: O and the sum are rescaled when a block's maximum
 // exceeds it by more than 8 (2^8 in P; f16: 2^15, as the maximum is held lower),
 // which keeps P within 16-bit range and the result exact, as both are taken
-// against the same maximum.
+// against the same maximum.  The sum takes the weights as the product does,
+// rounded: at 64 dims it is a column of that product (V beside a tile of ones,
+// N = 80), at 128, where no TMEM is left for it, 16-bit numbers added to f32 ones
+// (2 x 4092, 16 heads of 64, causal behind a prefix: error against 64 bits 1.26
+// times one rounding of the result's, 1.37 with the sum of the unrounded weights;
+// 141 -> 137 us; 16384 in 5 documents, 16 of 128: 1.11 and 1.18 times, 587 -> 596).
 //
 // Hidden places: a hidden score is replaced by -inf whatever it was, but a
 // hidden key's V still meets P = 0 in the product, and 0 * NaN is NaN.  So the
@@ -50,7 +55,7 @@ constexpr float kRescaleLog2 = 8.0f;
 constexpr int kSub = kN * 128;    // one 64-key x 64-dim operand tile, 128-byte rows
 constexpr int kTags = 8;          // unread tags: at most stages + 2
 constexpr uint32_t kTmemCols = 256;
-constexpr uint32_t kOCol = 128;   // S/P 0 (64) | S/P 1 (64) | O (up to 128)
+constexpr uint32_t kOCol = 128;   // S/P 0 (64) | S/P 1 (64) | O (up to 128; 64 dims: and the sum of weights)
 constexpr int kSmem = 100 * 1024;  // more than a third of an SM's: never a third CTA waiting for TMEM
 
 template <int D>
@@ -59,7 +64,13 @@ struct Cfg {
     static constexpr int Q_BYTES = SUBS * kM * 128;
     static constexpr int KV_BYTES = SUBS * kSub;
     static constexpr int STAGES = D == 64 ? 4 : 2;  // of K, and of V
-    static_assert(Q_BYTES + 2 * STAGES * KV_BYTES + 1024 + 512 + 4 * kN * 4 <= kSmem, "shared memory");
+    // The sum of weights: 64 dims leave TMEM columns for a product with ones (the
+    // 16 columns behind O); 128 dims fill them, and the softmax threads add up.
+    static constexpr bool ONES = D == 64;
+    static constexpr int ONES_BYTES = ONES ? kSub : 0;
+    static constexpr uint32_t L_COL = kOCol + D;
+    static_assert(Q_BYTES + 2 * STAGES * KV_BYTES + ONES_BYTES + 1024 + 512 + 4 * kN * 4 <= kSmem, "shared memory");
+    static_assert(!ONES || L_COL + 16 <= kTmemCols, "TMEM");
     static_assert(STAGES + 2 <= kTags, "tag ring");
 };
 
@@ -78,6 +89,19 @@ __device__ __forceinline__ float row_min64(const float (&s)[64]) {
         m[c] = fminf(m[c], s[60 + c]);
     }
     return fminf(min3f(m[0], m[1], m[2]), m[3]);
+}
+
+// a += the low, b += the high half of a packed pair.
+template <typename T>
+__device__ __forceinline__ void add_pair(float &a, float &b, uint32_t w) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tadd.rn.f32.bf16 %0, lo, %0;\n\tadd.rn.f32.bf16 %1, hi, %1;\n\t}"
+            : "+f"(a), "+f"(b)
+            : "r"(w));
+    else
+        asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tadd.rn.f32.f16 %0, lo, %0;\n\tadd.rn.f32.f16 %1, hi, %1;\n\t}"
+            : "+f"(a), "+f"(b)
+            : "r"(w));
 }
 
 // Infinities and NaN of a packed pair set to zero.
@@ -207,7 +231,8 @@ __global__ void __launch_bounds__(kThreadsF, 2)
     uint8_t *sQ = smem_raw + (((raw + 1023u) & ~1023u) - raw);
     uint8_t *sK = sQ + C::Q_BYTES;
     uint8_t *sV = sK + ST * C::KV_BYTES;
-    uint64_t *q_full = reinterpret_cast<uint64_t *>(sV + ST * C::KV_BYTES);
+    uint8_t *sOnes = sV + ST * C::KV_BYTES;
+    uint64_t *q_full = reinterpret_cast<uint64_t *>(sOnes + C::ONES_BYTES);
     uint64_t *k_full = q_full + 1, *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST;
     uint64_t *s_full = v_empty + ST, *p_full = s_full + 2, *pv_done = p_full + 2, *done_bar = pv_done + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done_bar + 1);
@@ -309,6 +334,12 @@ __global__ void __launch_bounds__(kThreadsF, 2)
         }
         if (lane == 0) *any_seen = cur >= 0;
     }
+    if constexpr (C::ONES) {
+        const uint32_t one2 = std::is_same<T, __nv_bfloat16>::value ? 0x3F803F80u : 0x3C003C00u;
+        for (int e = threadIdx.x; e < C::ONES_BYTES / 16; e += kThreadsF)
+            reinterpret_cast<uint4 *>(sOnes)[e] = make_uint4(one2, one2, one2, one2);
+        fence_proxy_async_smem();
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -373,7 +404,7 @@ __global__ void __launch_bounds__(kThreadsF, 2)
         // --------------------------------------------------------------- MMA
         if (lane == 0) {
             constexpr uint32_t idesc_s = idesc_f32acc(kM, kN, kBf16);
-            constexpr uint32_t idesc_o = idesc_f32acc(kM, D, kBf16, true);
+            constexpr uint32_t idesc_o = idesc_f32acc(kM, C::ONES ? D + 16 : D, kBf16, true);
             const uint32_t q_addr = smem_u32(sQ);
             bool ok = mbar_wait(q_full, 0, p.fault);
             auto issue_pv = [&](int i) -> bool {
@@ -381,9 +412,11 @@ __global__ void __launch_bounds__(kThreadsF, 2)
                 if (!mbar_wait(&v_full[st], (i / ST) & 1, p.fault) || !mbar_wait(&p_full[b], (i >> 1) & 1, p.fault)) return false;
                 tc_fence_after();
                 const uint32_t v_addr = smem_u32(sV + st * C::KV_BYTES);
+                // columns 64 on of the V operand: the second half of its dims, or the ones
+                const uint32_t next = C::ONES ? smem_u32(sOnes) - v_addr : kSub;
 #pragma unroll
                 for (int kk = 0; kk < kN / 16; ++kk)  // 16 keys: 8 packed TMEM columns of P, 2048 bytes of V
-                    umma_f16_ts(tmem + kOCol, tmem + b * kN + kk * 8, sw128_desc_mn(v_addr + kk * 2048, kSub), idesc_o,
+                    umma_f16_ts(tmem + kOCol, tmem + b * kN + kk * 8, sw128_desc_mn(v_addr + kk * 2048, next), idesc_o,
                             (i > 0 || kk > 0) ? 1u : 0u);
                 umma_commit(&pv_done[b]);
                 umma_commit(&v_empty[st]);
@@ -427,7 +460,7 @@ __global__ void __launch_bounds__(kThreadsF, 2)
         };
         const NearCap near(p.c0, p.c1);
         float m_run = -INFINITY;
-        F2 l2(0.0f, 0.0f);
+        float l0 = 0.0f, l1 = 0.0f;  // 128 dims: the sum of weights, even and odd keys
         bool ok = true;
         auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {  // warp-uniform: tcgen05.ld/st follow
             int r = 1;
@@ -543,8 +576,14 @@ __global__ void __launch_bounds__(kThreadsF, 2)
                         for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(o[e] * alpha);
                         tmem_st32(tmem + lane_base + kOCol + c, r);
                     }
+                    if constexpr (C::ONES) {
+                        float l = tmem_ld1(tmem + lane_base + C::L_COL);
+                        tmem_ld_wait_reg(l);
+                        tmem_st1(tmem + lane_base + C::L_COL, l * alpha);
+                    }
                     tmem_st_wait();
-                    l2 = mul2(l2, F2(alpha, alpha));
+                    l0 *= alpha;
+                    l1 *= alpha;
                 }
                 // a row that has seen no key yet has nothing to subtract: its weights are 2^-inf
                 const float nm = m_run == -INFINITY ? 0.0f : -m_run;
@@ -553,8 +592,8 @@ __global__ void __launch_bounds__(kThreadsF, 2)
                     x.get(x0, x1);
                     x0 = ex2f(x0);
                     x1 = ex2f(x1);
-                    l2 = add2(l2, F2(x0, x1));
                     pk[e] = pack2<T>(x0, x1);
+                    if constexpr (!C::ONES) add_pair<T>(l0, l1, pk[e]);
                 };
                 if (CAP && !BIAS && folded) {
 #pragma unroll
@@ -605,9 +644,11 @@ __global__ void __launch_bounds__(kThreadsF, 2)
         if (ok) ok = wait(&pv_done[i & 1], (i >> 1) & 1);
         tc_fence_after();
         asm volatile("bar.sync 1, 128;" ::: "memory");  // every softmax warp has noted its blocks
-        float l0, l1;
-        l2.get(l0, l1);
-        const float l = l0 + l1;
+        float l = l0 + l1;
+        if constexpr (C::ONES) {
+            l = tmem_ld1(tmem + lane_base + C::L_COL);
+            tmem_ld_wait_reg(l);
+        }
         const float inv = p.splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
         const int64_t part = ((sr.q0 + static_cast<int64_t>(row0) + row) * p.heads + head) * p.splits + split;
         if (p.splits > 1 && ok && valid) p.part_ml[part] = make_float2(m_run, l);

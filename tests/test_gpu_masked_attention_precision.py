@@ -93,3 +93,24 @@ def test_f16_weights_far_below_the_largest(lq, n, d):
     tol = want * (rel + 2.0 ** -11) * 1.01 + 2.0 ** -25
     err = (got.double().reshape(lq, 2, d) - want).abs()
     assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.parametrize("d,dtype", [(64, HF), (64, BF), (128, HF), (128, BF)])
+@pytest.mark.parametrize("lq,n", [(1, 100), (7, 90), (8, 1400), (200, 300), (64, 1500), (900, 900)])
+@pytest.mark.parametrize("rules", [dict(), dict(causal=True, softcap=50.0)])
+def test_values_that_are_alike_average_to_themselves(lq, n, d, dtype, rules):
+    """Whatever the weights are, a weighted mean of equal numbers is that number:
+    the weights are summed as the product with V takes them.  f32 sums of n <=
+    1500 terms are n 2^-24 off, below half a step of the result."""
+    o = ops()
+    q, k, v = (torch.zeros((m, 2 * d), device="cuda") for m in (lq, n, n))
+    q[:, 0] = q[:, d] = torch.linspace(0.1, 3.0, lq, device="cuda")
+    q[:, 1] = q[:, d + 1] = torch.linspace(0.0, 0.01, lq, device="cuda")
+    k[:, 0] = k[:, d] = -1
+    k[:, 1] = k[:, d + 1] = torch.linspace(-1, 1, n, device="cuda")
+    k[0] = 0
+    v[:] = torch.rand((1, 2 * d), device="cuda", generator=torch.Generator(device="cuda").manual_seed(d)) * 4 - 2
+    q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+    got = o.masked_attention(q, k, v, cu([lq]), cu([n]), lq, n, 2, 1.0, **rules)
+    o.ctx().sync_check()
+    assert torch.equal(got, v[:1].expand_as(got)), float((got.double() / v[0].double() - 1).abs().max())
