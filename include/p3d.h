@@ -260,8 +260,9 @@ int p3d_quantize_rows(p3d_ctx *ctx, const void *x, int64_t ldx, int64_t m, int64
  * x [m][ldx] and w [n][ldw] signed 8-bit (-128 included), 16-byte aligned,
  * ldx and ldw multiples of 16 (k itself may be any size up to 131071; bytes
  * from k on are not used); x_scale f32 [m], w_scale f32 [n], bias f32 [n] or
- * NULL.  out, epilogue, gate and batch offsets as in p3d_linear; with 16-bit
- * out GELU takes the hardware tanh, with f32 out it is accurate to f32. */
+ * NULL.  out, epilogue, gate and batch offsets as in p3d_linear, but GELU is
+ * right to a few 2^-22 of its own value before out's rounding (p3d_linear's is
+ * up to 2^-12 |x| off, from the hardware tanh). */
 int p3d_linear_i8(p3d_ctx *ctx, const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *w, int64_t ldw,
                   const float *w_scale, const float *bias, int64_t m, int64_t n, int64_t k, void *out, int64_t ldo,
                   int out_dtype, int epilogue, const float *gate, int64_t gate_ld, const int32_t *batch_offsets,

@@ -16,14 +16,15 @@
 // accumulators in TMEM, so a tile's epilogue runs under the next one's MMAs.
 // Every wait is bounded.
 //
-// What bounds it, 8184 x 1024 x 4096 to bf16 (68.6 Gop): 33.1 us = 2070 Top/s,
-// with GELU 35.0; the MMAs alone take 22.5 us (3055 Top/s), with their loads
+// What bounds it, 8184 x 1024 x 4096 to bf16 (68.6 Gop): 33.3 us = 2060 Top/s,
+// with GELU 38.3; the MMAs alone take 22.5 us (3055 Top/s), with their loads
 // 24.8.  The rest is the epilogue's share of shared memory and issue slots,
-// which at K = 1024 is one pass over 64 KB for eight stages.  Eight epilogue
-// warps instead of 16 took 43.1 us with GELU (their loads' latency showed),
-// 4 KB staging slots and so three stages instead of four 37.7.  CTA pairs
-// (cta_group::2, half the loads of w) were slower here (35.4, 38.3 with GELU)
-// and 2 % faster at 8184 x 4096 x 4096 (101.0 / 102.7 us), so there are none.
+// which at K = 1024 is one pass over 64 KB for eight stages.  Tried where GELU
+// took the hardware tanh (35.0 us): eight epilogue warps instead of 16 43.1 us
+// (their loads' latency showed), 4 KB staging slots and so three stages instead
+// of four 37.7, CTA pairs (cta_group::2, half the loads of w) 38.3 (without GELU
+// 35.4 against 33.1) and 2 % faster at 8184 x 4096 x 4096 (101.0 / 102.7 us), so
+// there are none.
 #include <algorithm>
 #include <cstring>
 
@@ -51,17 +52,16 @@ struct I8Params {
     int wide_cols;  // w_scale and bias start on 16-byte boundaries
 };
 
-// GELU, tanh form, for f32 outputs: x sigmoid(2 y), a few 2^-23 of the result
-// and of its slope (the hardware tanh would be 2^-11 off).
-__device__ __forceinline__ float gelu_f32_f(float x) {
+// GELU, tanh form, as x sigmoid(2 y): a few 2^-23 of the result and of its slope.
+// (0.5 x (1 + tanh(y)) by the hardware tanh is 2^-12 |x| off wherever the two
+// cancel: 20 % of the value at x = -3, in 16 bits too.)
+__device__ __forceinline__ float gelu_f(float x) {
     const float y = 0.7978845608028654f * fmaf(0.044715f * x, x * x, x);
     return __fdividef(x, 1.0f + __expf(-2.0f * y));
 }
 
-// Activation of one value: 16-bit outputs take the hardware tanh (relative
-// error about 2^-11, half a step of f16), f32 outputs the exact forms.
-__device__ __forceinline__ float act_f(float v, int epi, int out_dtype) {
-    if (epi & P3D_EPI_GELU_TANH) return out_dtype == P3D_F32 ? gelu_f32_f(v) : gelu_tanh_f(v);
+__device__ __forceinline__ float act_f(float v, int epi) {
+    if (epi & P3D_EPI_GELU_TANH) return gelu_f(v);
     if (epi & P3D_EPI_SILU) return silu_f(v);
     return v;
 }
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kRowThreads) linear_i8_rows_kernel(const I8Par
     if (r < rows && c < cols) {
         const int64_t row = row0 + r, col = col0 + c;
         const float bias = p.bias ? p.bias[col] : 0.0f;
-        store_one(p, row, col, act_f(fmaf(static_cast<float>(mine) * p.xs[row], p.ws[col], bias), p.epi, p.out_dtype));
+        store_one(p, row, col, act_f(fmaf(static_cast<float>(mine) * p.xs[row], p.ws[col], bias), p.epi));
     }
 }
 
@@ -197,16 +197,22 @@ struct TileCfg {
     static_assert(TMEM == 128 || TMEM == 256 || TMEM == 512, "TMEM columns");
 };
 
-// Two values of GELU by the hardware tanh (gelu_tanh_f).
+// Two values of gelu_f for 16-bit outputs: the exponential and the reciprocal
+// approximate, 2^-21 of the result together (8184 x 1024 x 4096 to bf16: 38.3 us;
+// one reciprocal for both 37.8, a cubic and a Newton step in its place 39.1, the
+// hardware tanh 34.8).
 __device__ __forceinline__ F2 gelu2(const F2 &x) {
-    constexpr float c0 = 0.7978845608028654f, c1 = c0 * 0.044715f;
+    constexpr float c0 = -2.0f * 1.4426950408889634f * 0.7978845608028654f, c1 = c0 * 0.044715f;
     const F2 y = mul2(fma2(mul2(x, x), F2(c1, c1), F2(c0, c0)), x);
     float a, b;
     y.get(a, b);
-    asm("tanh.approx.f32 %0, %0;" : "+f"(a));
-    asm("tanh.approx.f32 %0, %0;" : "+f"(b));
-    const F2 h = mul2(x, F2(0.5f, 0.5f));
-    return fma2(h, F2(a, b), h);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+    const F2 d = add2(F2(a, b), F2(1.0f, 1.0f));
+    d.get(a, b);
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
+    return mul2(x, F2(a, b));
 }
 
 // 32 accumulators of one row to outputs, columns col0.. (ncols of them exist).
@@ -255,7 +261,7 @@ __device__ __forceinline__ void finish32(const I8Params &p, float (&v)[32], floa
     }
     if ((p.epi & P3D_EPI_GELU_TANH) && !fast_gelu) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = gelu_f32_f(v[i]);
+        for (int i = 0; i < 32; ++i) v[i] = gelu_f(v[i]);
     } else if (p.epi & P3D_EPI_SILU) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = silu_f(v[i]);

@@ -260,3 +260,34 @@ def test_refusals():
     q, s = o.quantize_rows(f[:0])
     assert q.shape == (0, 32) and s.shape == (0,)
     assert o.linear_i8(x[:0], a[:0], w, b).shape == (0, 8)
+
+
+@pytest.mark.parametrize("out_dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(2, 900, 64), (5, 5000, 40), (400, 700, 100), (1300, 1024, 96)])
+def test_linear_i8_gelu_is_right_to_a_step_everywhere(m, n, k, out_dtype):
+    """GELU between -10 and 4 against its own size: its values left of -2 are small,
+    and a small one's sign and size are as good as a large one's."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    pitch = (k + 15) // 16 * 16
+    x = torch.randint(-20, 21, (m, pitch), device="cuda", generator=g).to(torch.int8)[:, :k]
+    w = torch.randint(-20, 21, (n, pitch), device="cuda", generator=g).to(torch.int8)[:, :k]
+    xs, ws = torch.rand(m, device="cuda", generator=g) + 0.5, torch.full((n,), 1.0 / (1500 * math.sqrt(k)), device="cuda")
+    b = torch.linspace(-10, 4, n, device="cuda")
+    got = ops().linear_i8(x, xs, w, ws, b, out_dtype=out_dtype, epilogue=L().EPI_GELU_TANH)
+    y = x.double() @ w.double().t() * xs.double()[:, None] * ws.double()
+    size, c = y.abs(), math.sqrt(2 / math.pi)
+    p = (y + b.double()).requires_grad_()
+    z = 2 * c * (p + 0.044715 * p ** 3)
+    want = p * torch.sigmoid(z)
+    slope = torch.autograd.grad(want.sum(), p)[0].abs()
+    p, z, want = p.detach(), z.detach(), want.detach()
+    # the argument: three roundings of the product and one of the sum, carried by the slope (and its
+    # change over that little distance: below 2 times its square).  The form x / (1 + exp(-z)): z is off
+    # by five roundings of itself (2^-24 each) of which exp makes |z| times as much, the exponential's 2^-22 and its
+    # own argument's rounding, the division's 2^-22; denominators past 2^126 count as infinite
+    dp = 2.0 ** -24 * (3 * size + p.abs()) * 1.01
+    tol = slope * dp + 2 * dp ** 2 + want.abs() * 2.0 ** -22 * (4 + 2 * z.abs()) + p.abs() * 2.0 ** -125
+    u = torch.finfo(out_dtype).eps / 2 if out_dtype != torch.float32 else 0.0
+    tol = tol + u * (want.abs() + tol) + (2.0 ** -25 if out_dtype == torch.float16 else 0.0)
+    err = (got.double() - want).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
