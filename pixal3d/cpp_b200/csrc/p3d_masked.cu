@@ -160,14 +160,15 @@ struct TilePlan {
     int64_t tiles;
     bool ordered;
     size_t docs, order, o, ml;
-    TilePlan(int nseq, int64_t max_q, int64_t max_k, int64_t rows_q, int64_t rows_k, int heads, int head_dim, bool documents) {
+    TilePlan(int nseq, int64_t max_q, int64_t max_k, int64_t rows_k, int heads, int head_dim, bool documents) {
         const int64_t ctas = static_cast<int64_t>(heads) * nseq * ceil_div(max_q, 128);
         splits = ctas > 148 ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({296 / std::max<int64_t>(ctas, 1), max_k / 512, 16})));
         tiles = nseq * ceil_div(max_q, 128);
         ordered = documents && ctas > 296 && tiles <= kOrderTiles;
         order = ordered ? align256(static_cast<size_t>(2 * tiles + 1) * sizeof(int4)) : 0;
         docs = documents ? align256(static_cast<size_t>(rows_k / 64 + nseq + 1) * sizeof(int2)) : 0;
-        const size_t parts = splits > 1 ? static_cast<size_t>(rows_q) * heads * splits : 0;
+        // at most 296 x 128 rows, whatever rows q has beside the sequences'
+        const size_t parts = splits > 1 ? static_cast<size_t>(nseq) * max_q * heads * splits : 0;
         o = align256(parts * head_dim * sizeof(float));
         ml = align256(parts * sizeof(float2));
     }
@@ -182,7 +183,7 @@ extern "C" size_t p3d_masked_attention_workspace(int nseq, int64_t max_q, int64_
                                                  int heads, int kv_heads, int head_dim, int documents) {
     if (nseq <= 0 || max_q <= 0 || max_k < 0 || rows_q <= 0 || rows_k < 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
     if (max_q > kFewRows) {
-        const TilePlan plan(nseq, max_q, max_k, rows_q, rows_k, heads, head_dim, documents != 0);
+        const TilePlan plan(nseq, max_q, max_k, rows_k, heads, head_dim, documents != 0);
         return plan.docs + plan.order + plan.o + plan.ml;
     }
     if (max_k <= kFewKeys) return 0;
@@ -258,7 +259,7 @@ extern "C" int p3d_masked_attention(p3d_ctx *ctx, const void *q, int64_t ldq, co
     p.fault = ctx->fault;
     DeviceGuard on(ctx->device);
     if (max_q > kFewRows && rows_k > 0) {
-        const TilePlan plan(nseq, max_q, max_k, rows_q, rows_k, heads, head_dim, r.doc_k != nullptr);
+        const TilePlan plan(nseq, max_q, max_k, rows_k, heads, head_dim, r.doc_k != nullptr);
         char *at = static_cast<char *>(ws);
         p.splits = plan.splits;
         p.doc_range = reinterpret_cast<int2 *>(at);

@@ -24,7 +24,7 @@ struct MaskedParams {
     // against their own maxima, and (maximum, sum)
     int item_rows, piece, blocks;
     int64_t parts;
-    int splits;  // many queries: of the key blocks; results [row * heads + head][split]
+    int splits;  // many queries: of the key blocks; results [(sequence, query), head][split]
     float *part_o;
     float2 *part_ml;
     int2 *doc_range; // (smallest, largest) document number of every 64-key block

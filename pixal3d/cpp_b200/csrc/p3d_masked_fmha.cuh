@@ -198,6 +198,12 @@ __device__ __forceinline__ void bias_row(float (&s)[64], float scale, float slop
     }
 }
 
+// First of the splits' results of query qi (below max_q) of a sequence: by the
+// sequence's place, not by the row, since q may hold many more rows.
+__device__ __forceinline__ int64_t split_part(const MaskedParams &p, int seq, int64_t qi, int head) {
+    return ((seq * p.max_q + qi) * p.heads + head) * p.splits;
+}
+
 template <typename T, int D, bool CAP, bool BIAS, bool DOCS>
 __global__ void __launch_bounds__(kThreadsF, 2)
     masked_fmha_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -350,7 +356,7 @@ __global__ void __launch_bounds__(kThreadsF, 2)
 
     if (nothing && p.splits > 1) {
         for (int e = threadIdx.x; e < nrows; e += kThreadsF)
-            p.part_ml[((sr.q0 + static_cast<int64_t>(row0) + e) * p.heads + head) * p.splits + split] = make_float2(-INFINITY, 0.0f);
+            p.part_ml[split_part(p, seq, row0 + e, head) + split] = make_float2(-INFINITY, 0.0f);
     } else if (nothing) {
         T *o = static_cast<T *>(p.out) + (sr.q0 + static_cast<int64_t>(row0)) * p.ldo + static_cast<int64_t>(head) * D;
         for (int e = threadIdx.x; e < nrows * (D / 8); e += kThreadsF)
@@ -650,7 +656,7 @@ __global__ void __launch_bounds__(kThreadsF, 2)
             tmem_ld_wait_reg(l);
         }
         const float inv = p.splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-        const int64_t part = ((sr.q0 + static_cast<int64_t>(row0) + row) * p.heads + head) * p.splits + split;
+        const int64_t part = split_part(p, seq, row0 + row, head) + split;
         if (p.splits > 1 && ok && valid) p.part_ml[part] = make_float2(m_run, l);
         const int bad0 = bad[0], bad1 = bad[1];
         T *dst = static_cast<T *>(p.out) + (sr.q0 + static_cast<int64_t>(row0) + row) * p.ldo + static_cast<int64_t>(head) * D;
@@ -708,7 +714,7 @@ __global__ void __launch_bounds__(256) masked_splits_kernel(const MaskedParams p
     const int64_t qi = item / p.heads;
     const SeqRange sr = seq_range(p, blockIdx.y);
     if (qi >= sr.lq || qi >= p.max_q) return;
-    const int64_t at = ((sr.q0 + qi) * p.heads + head) * p.splits;
+    const int64_t at = split_part(p, blockIdx.y, qi, head);
     const float mine = lane < p.splits ? p.part_ml[at + lane].x : -INFINITY;
     float mm = mine;
 #pragma unroll

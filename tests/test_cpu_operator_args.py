@@ -43,3 +43,13 @@ def test_rotary_frequencies_on_the_host():
     assert torch.allclose(f, 10.0 ** -torch.tensor([0, 0.25, 0.5, 0.75], dtype=torch.float64), rtol=1e-15, atol=0)
     with pytest.raises(ValueError):
         ops.rotary_frequencies(8, fast=1.0, slow=1.0, device="cpu")
+
+
+def test_masked_attention_workspace_does_not_grow_with_spare_query_rows():
+    """64 queries over 8192 keys, split between blocks, in a q of 64 rows and of
+    32768: the same results to join, so the same workspace."""
+    ws = L.lib.p3d_masked_attention_workspace
+    for documents in (0, 1):
+        assert 0 < ws(1, 64, 8192, 32768, 8192, 16, 16, 128, documents) == ws(1, 64, 8192, 64, 8192, 16, 16, 128, documents)
+    for nseq, max_q, heads in ((1, 9, 1), (1, 2000, 4), (3, 200, 6), (100, 100, 1)):
+        assert ws(nseq, max_q, 16384, 1 << 30, 16384 * nseq, heads, heads, 128, 0) <= 296 * 128 * (128 + 2) * 4 + 512

@@ -520,3 +520,10 @@ def test_caps_near_and_far_from_the_scores(d, dtype, causal):
     """Blocks whose scores all lie within half the cap, blocks with a row beyond it, and the largest score on either side of it."""
     for softcap, sharp in ((50.0, 1.0), (50.0, 6.0), (8.0, 1.0), (3.0, 0.3), (1000.0, 4.0)):
         run([(300, 300), (140, 500)], 4, 2, d, dtype, softcap=softcap, sharp=sharp, causal=causal)
+
+
+@pytest.mark.parametrize("d,dtype", [(64, HF), (128, BF)])
+def test_split_keys_in_longer_buffers(d, dtype):
+    """Splits are joined by the sequences' places, whatever rows lie behind them."""
+    run([(64, 5000), (30, 700), (0, 9), (9, 2)], 4, 2, d, dtype, causal=True, spare=3000)
+    run([(1, 30), (100, 4000)], 6, 3, d, dtype, slopes=torch.rand(6, device="cuda"), spare=500)
