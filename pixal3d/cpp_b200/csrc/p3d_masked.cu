@@ -119,7 +119,7 @@ int masked_attention_tiles(p3d_ctx *ctx, const MaskedParams &p, int head_dim, in
 // head's queries and heads), 16-key tiles of a piece, blocks, pieces at most,
 // and the bytes of their results.
 struct PiecePlan {
-    int item_rows, piece, blocks;
+    int item_rows, piece, most_pieces, blocks;
     int64_t parts;
     size_t o, ml;
     PiecePlan(int nseq, int64_t max_q, int64_t max_k, int64_t rows_k, int heads, int kv_heads, int head_dim) {
@@ -144,8 +144,10 @@ struct PiecePlan {
                 piece = static_cast<int>(l);
             }
         }
-        blocks = static_cast<int>(std::min<int64_t>(148, nseq * items * ceil_div(std::max<int64_t>(max_k, 1), 16 * static_cast<int64_t>(piece))));
-        parts = items * ((rows_k / 16 + nseq) / piece + nseq);
+        most_pieces = static_cast<int>(ceil_div(std::max<int64_t>(max_k, 1), 16 * static_cast<int64_t>(piece)));
+        blocks = static_cast<int>(std::min<int64_t>(148, nseq * items * most_pieces));
+        // of all sequences: by their number, or by the rows that they share
+        parts = items * std::min(static_cast<int64_t>(nseq) * most_pieces, (rows_k / 16 + nseq) / piece + nseq);
         o = align256(static_cast<size_t>(parts) * item_rows * head_dim * sizeof(float));
         ml = align256(static_cast<size_t>(parts) * item_rows * sizeof(float2));
     }
@@ -278,6 +280,7 @@ extern "C" int p3d_masked_attention(p3d_ctx *ctx, const void *q, int64_t ldq, co
     const PiecePlan plan(nseq, max_q, max_k, rows_k, heads, kv_heads, head_dim);
     p.item_rows = plan.item_rows;
     p.piece = plan.piece;
+    p.most_pieces = plan.most_pieces;
     p.blocks = plan.blocks;
     p.parts = plan.parts;
     p.part_o = static_cast<float *>(ws);

@@ -20,9 +20,9 @@ struct MaskedParams {
     const float *slopes;
     int head_tiles;  // few keys: groups of 8 or 16 heads of a K/V head
     // few queries, long keys: rows (query, head) of an item, key tiles of a
-    // piece, blocks, and the pieces' results: [parts][item_rows][D] sums
-    // against their own maxima, and (maximum, sum)
-    int item_rows, piece, blocks;
+    // piece, pieces of an item at most, blocks, and the pieces' results:
+    // [parts][item_rows][D] sums against their own maxima, and (maximum, sum)
+    int item_rows, piece, most_pieces, blocks;
     int64_t parts;
     int splits;  // many queries: of the key blocks; results [(sequence, query), head][split]
     float *part_o;

@@ -66,15 +66,21 @@ __device__ __forceinline__ int seq_rows(const MaskedParams &p, const SeqRange &s
 __device__ __forceinline__ int seq_items(const MaskedParams &p, const SeqRange &sr) {
     return (seq_rows(p, sr) + p.item_rows - 1) / p.item_rows * p.kv_heads;
 }
+// Pieces of an item, and their tiles: p.piece, or, in a sequence longer than
+// max_k, as many as leave it no more pieces than one of max_k keys has (the
+// results' space is of that many; the last ones may be empty).
 __device__ __forceinline__ int item_pieces(const MaskedParams &p, const SeqRange &sr) {
-    return (item_tiles(sr) + p.piece - 1) / p.piece;
+    return min((item_tiles(sr) + p.piece - 1) / p.piece, p.most_pieces);
+}
+__device__ __forceinline__ int piece_tiles(const MaskedParams &p, const SeqRange &sr) {
+    return max(p.piece, (item_tiles(sr) + p.most_pieces - 1) / p.most_pieces);
 }
 
 // Places in the order of all pieces (whole warps call these).
 struct Walk {
     int64_t u = 0, before = 0;  // the piece, and the pieces before its sequence
     SeqRange sr;
-    int seq = 0, items = 0, pieces = 0;
+    int seq = 0, items = 0, pieces = 0, length = 0;
     int item, t, take;  // of the piece: its item, first key tile, tiles
     bool whole;         // the item's only piece
 
@@ -101,6 +107,7 @@ struct Walk {
                 sr = seq_range(p, seq);
                 items = seq_items(p, sr);
                 pieces = item_pieces(p, sr);
+                length = piece_tiles(p, sr);
                 return true;
             }
             before += __shfl_sync(0xffffffffu, upto, 31);
@@ -113,8 +120,8 @@ struct Walk {
         if (u >= before + static_cast<int64_t>(items) * pieces && !find(p, lane)) return false;
         const int in = static_cast<int>(u - before);
         item = in % items;
-        t = in / items * p.piece;
-        take = min(p.piece, item_tiles(sr) - t);
+        t = in / items * length;
+        take = max(min(length, item_tiles(sr) - t), 0);
         whole = pieces == 1;
         return true;
     }

@@ -53,3 +53,10 @@ def test_masked_attention_workspace_does_not_grow_with_spare_query_rows():
         assert 0 < ws(1, 64, 8192, 32768, 8192, 16, 16, 128, documents) == ws(1, 64, 8192, 64, 8192, 16, 16, 128, documents)
     for nseq, max_q, heads in ((1, 9, 1), (1, 2000, 4), (3, 200, 6), (100, 100, 1)):
         assert ws(nseq, max_q, 16384, 1 << 30, 16384 * nseq, heads, heads, 128, 0) <= 296 * 128 * (128 + 2) * 4 + 512
+
+
+def test_masked_attention_workspace_does_not_grow_with_spare_key_rows():
+    """One token over 1024 keys that lie in a cache of 2^20 rows: as over 1024."""
+    ws = L.lib.p3d_masked_attention_workspace
+    assert 0 < ws(1, 1, 1024, 1, 1 << 20, 32, 8, 128, 0) <= ws(1, 1, 1024, 1, 1024, 32, 8, 128, 0)
+    assert 0 < ws(4, 2, 3000, 9, 1 << 24, 32, 8, 64, 0) <= ws(4, 2, 3000, 9, 4 * 3000, 32, 8, 64, 0)

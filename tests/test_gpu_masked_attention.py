@@ -527,3 +527,20 @@ def test_split_keys_in_longer_buffers(d, dtype):
     """Splits are joined by the sequences' places, whatever rows lie behind them."""
     run([(64, 5000), (30, 700), (0, 9), (9, 2)], 4, 2, d, dtype, causal=True, spare=3000)
     run([(1, 30), (100, 4000)], 6, 3, d, dtype, slopes=torch.rand(6, device="cuda"), spare=500)
+
+
+@pytest.mark.parametrize("d,dtype", [(64, HF), (128, BF)])
+def test_sequences_longer_than_max_k(d, dtype):
+    """A max_k below the longest sequence costs time only, and a cache of many
+    more rows than the sequences have costs nothing."""
+    o = ops()
+    lens = [(1, 40000), (3, 700), (2, 5000), (1, 0), (1, 9)]
+    nq, nk = sum(a for a, _ in lens), sum(b for _, b in lens)
+    g = torch.Generator(device="cuda").manual_seed(17)
+    q = torch.randn((nq, 8 * d), device="cuda", generator=g).to(dtype)
+    k, v = (torch.randn((nk + 100000, 2 * d), device="cuda", generator=g).to(dtype) for _ in range(2))
+    want, tol = attention64(q, k, v, lens, 8, 2, 0.1, causal=True)
+    for max_k in (513, 600, 3000, 40000):
+        got = o.masked_attention(q, k, v, cu([a for a, _ in lens]), cu([b for _, b in lens]), 3, max_k, 8, 0.1, kv_heads=2, causal=True)
+        o.ctx().sync_check()
+        assert bool(((got.double() - want).abs() <= tol).all()), max_k
