@@ -72,6 +72,11 @@ typedef struct p3d_ctx p3d_ctx;
  * expect ctx's device to be current (as CUDA runtime calls do); the
  * p3d_flow_* entry points make it current themselves for their duration. */
 int p3d_ctx_create(int device, void *stream, p3d_ctx **out);
+/* Another context on ctx's device, for another host thread or object: its own
+ * stream, error message and place in calls, so that the two never mix, but
+ * ctx's fault flag and launch count.  Allocates nothing on the device (it may be
+ * made during a stream capture).  Destroy it before ctx. */
+int p3d_ctx_fork(p3d_ctx *ctx, void *stream, p3d_ctx **out);
 int p3d_ctx_destroy(p3d_ctx *ctx);
 int p3d_ctx_set_stream(p3d_ctx *ctx, void *stream);
 void *p3d_ctx_stream(const p3d_ctx *ctx);
@@ -79,7 +84,7 @@ void *p3d_ctx_stream(const p3d_ctx *ctx);
 const char *p3d_last_error(const p3d_ctx *ctx);
 /* Synchronize the stream and report (then clear) the device fault flag. */
 int p3d_ctx_check(p3d_ctx *ctx);
-/* Number of kernels this library launched on ctx since creation. */
+/* Number of kernels this library launched on ctx and its forks since creation. */
 int64_t p3d_ctx_launch_count(const p3d_ctx *ctx);
 int p3d_version(void);
 

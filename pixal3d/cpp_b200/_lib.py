@@ -111,6 +111,7 @@ def _sig(name, res, *args):
 
 _sig("p3d_version", i32)
 _sig("p3d_ctx_create", i32, i32, vp, C.POINTER(vp))
+_sig("p3d_ctx_fork", i32, vp, vp, C.POINTER(vp))
 _sig("p3d_ctx_destroy", i32, vp)
 _sig("p3d_ctx_set_stream", i32, vp, vp)
 _sig("p3d_ctx_stream", vp, vp)

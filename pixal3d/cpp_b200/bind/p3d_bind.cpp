@@ -5,7 +5,8 @@
 // stream and the call take about 4.  ops.py documents the functions and calls
 // them by position; the checks are theirs: ValueError and TypeError for
 // tensors that do not fit, P3DError for a status of the library.  The calls
-// go to the same libp3dcuda.so contexts as the ctypes binding's.
+// go through contexts of libp3dcuda.so that share the ctypes binding's fault
+// flags and launch counts.
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
@@ -14,7 +15,6 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
-#include <mutex>
 #include <string>
 
 #include "p3d.h"
@@ -25,10 +25,18 @@ using at::ScalarType;
 using at::Tensor;
 
 constexpr int kMaxDevices = 64;
-p3d_ctx *g_ctx[kMaxDevices] = {};
-PyObject *g_make_context = nullptr;  // (device) -> handle
+PyObject *g_root_context = nullptr;  // (device) -> handle of the device's first context, which stays
 PyObject *g_error = nullptr;         // P3DError(status, message)
-std::mutex g_mutex;                  // a stream bound and used by one thread at a time
+
+// A host thread's contexts, forks of the devices' first ones: no other thread,
+// nor the ctypes binding, sets their stream.
+struct ThreadContexts {
+    p3d_ctx *of[kMaxDevices] = {};
+    ~ThreadContexts() {
+        for (p3d_ctx *c : of) p3d_ctx_destroy(c);
+    }
+};
+thread_local ThreadContexts t_contexts;
 
 struct Raised {};  // a Python error has been set
 
@@ -114,15 +122,16 @@ bool truth(PyObject *o) {
 
 p3d_ctx *context(int device, const char *what) {
     need(device < kMaxDevices, what, "device index out of range");
-    if (!g_ctx[device]) {
-        PyObject *h = PyObject_CallFunction(g_make_context, "i", device);
+    p3d_ctx *&mine = t_contexts.of[device];
+    if (!mine) {
+        PyObject *h = PyObject_CallFunction(g_root_context, "i", device);
         if (!h) throw Raised();
         void *p = PyLong_AsVoidPtr(h);
         Py_DECREF(h);
         if (!p) throw Raised();
-        g_ctx[device] = static_cast<p3d_ctx *>(p);
+        if (p3d_ctx_fork(static_cast<p3d_ctx *>(p), nullptr, &mine) != P3D_OK) fail(PyExc_MemoryError, what, "no context");
     }
-    return g_ctx[device];
+    return mine;
 }
 
 // call(ctx) on torch's current stream of the device, without the GIL.
@@ -133,12 +142,9 @@ void launch(int device, const char *what, F &&call) {
     int rc;
     std::string message;
     Py_BEGIN_ALLOW_THREADS;
-    {
-        std::lock_guard<std::mutex> turn(g_mutex);
-        p3d_ctx_set_stream(ctx, stream);
-        rc = call(ctx);
-        if (rc != P3D_OK) message = p3d_last_error(ctx);
-    }
+    p3d_ctx_set_stream(ctx, stream);
+    rc = call(ctx);
+    if (rc != P3D_OK) message = p3d_last_error(ctx);
     Py_END_ALLOW_THREADS;
     if (rc != P3D_OK) {
         PyObject *e = PyObject_CallFunction(g_error, "is", rc, message.c_str());
@@ -364,7 +370,7 @@ PyObject *masked_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     P3D_BIND_END
 }
 
-// make_context(device) -> handle, P3DError
+// root_context(device) -> handle, P3DError
 PyObject *setup(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     if (nargs != 2) {
         PyErr_SetString(PyExc_TypeError, "setup: 2 arguments wanted");
@@ -372,7 +378,7 @@ PyObject *setup(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     }
     Py_INCREF(a[0]);
     Py_INCREF(a[1]);
-    Py_XSETREF(g_make_context, a[0]);
+    Py_XSETREF(g_root_context, a[0]);
     Py_XSETREF(g_error, a[1]);
     Py_RETURN_NONE;
 }

@@ -15,6 +15,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 
 #include "p3d.h"
@@ -25,7 +26,13 @@ struct p3d_ctx {
     int num_sms = 148;
     int *fault = nullptr;  // device flag: first latched p3d_status
     std::string error;
-    int64_t launches = 0;
+    int64_t launches = 0;            // of this context
+    std::atomic<int64_t> total{0};   // root: of it and its forks
+    p3d_ctx *root = nullptr;         // fork: the context whose fault flag and total it shares
+    void count_launches(int64_t n) {
+        launches += n;
+        (root ? root : this)->total += n;
+    }
 };
 
 namespace p3d {

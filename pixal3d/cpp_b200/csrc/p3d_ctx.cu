@@ -1,5 +1,6 @@
 // Context, error reporting and precision conversions.
 #include <cstdio>
+#include <new>
 
 #include "p3d_common.cuh"
 
@@ -11,7 +12,7 @@ int set_error(p3d_ctx *ctx, int status, const std::string &msg) {
 }
 
 int check_launch(p3d_ctx *ctx, const char *what) {
-    ++ctx->launches;
+    ctx->count_launches(1);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return set_error(ctx, P3D_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
     return P3D_OK;
@@ -60,9 +61,22 @@ extern "C" int p3d_ctx_create(int device, void *stream, p3d_ctx **out) {
     return P3D_OK;
 }
 
+extern "C" int p3d_ctx_fork(p3d_ctx *ctx, void *stream, p3d_ctx **out) {
+    if (!ctx || !out) return P3D_ERR_INVALID;
+    p3d_ctx *fork = new (std::nothrow) p3d_ctx();
+    *out = fork;
+    if (!fork) return P3D_ERR_CUDA;
+    fork->device = ctx->device;
+    fork->stream = static_cast<cudaStream_t>(stream);
+    fork->num_sms = ctx->num_sms;
+    fork->fault = ctx->fault;
+    fork->root = ctx->root ? ctx->root : ctx;
+    return P3D_OK;
+}
+
 extern "C" int p3d_ctx_destroy(p3d_ctx *ctx) {
     if (!ctx) return P3D_OK;
-    if (ctx->fault) cudaFree(ctx->fault);
+    if (ctx->fault && !ctx->root) cudaFree(ctx->fault);
     delete ctx;
     return P3D_OK;
 }
@@ -77,7 +91,7 @@ extern "C" void *p3d_ctx_stream(const p3d_ctx *ctx) { return ctx ? ctx->stream :
 
 extern "C" const char *p3d_last_error(const p3d_ctx *ctx) { return ctx ? ctx->error.c_str() : "null context"; }
 
-extern "C" int64_t p3d_ctx_launch_count(const p3d_ctx *ctx) { return ctx ? ctx->launches : 0; }
+extern "C" int64_t p3d_ctx_launch_count(const p3d_ctx *ctx) { return ctx ? (ctx->root ? ctx->root : ctx)->total.load() : 0; }
 
 extern "C" int p3d_ctx_check(p3d_ctx *ctx) {
     if (!ctx) return P3D_ERR_INVALID;

@@ -1054,7 +1054,7 @@ extern "C" int p3d_flow_sample_concat(p3d_flow *f, float *x, const void *ctx_fea
         for (int s = first; s < cfg->steps; ++s) {
             if (cfg->use_graph && f->step_graph) {
                 P3D_CUDA(ctx, cudaGraphLaunch(f->step_graph, f->stream));
-                ctx->launches += f->launches_per_step;
+                ctx->count_launches(f->launches_per_step);
             } else {
                 const int64_t l0 = ctx->launches;
                 P3D_TRY(one_step());

@@ -15,7 +15,7 @@ import ctypes as C
 import torch
 
 from . import _lib as L
-from .ops import ctx as _ctx
+from .ops import new_ctx as _new_ctx
 
 _CONVNEXT = {"norm_w": "norm_w", "norm_b": "norm_b", "conv_w": "conv1_w", "conv_b": "conv1_b", "mlp0_w": "mlp0_w",
              "mlp0_b": "mlp0_b", "mlp2_w": "mlp2_w", "mlp2_b": "mlp2_b"}
@@ -71,7 +71,7 @@ class Decoder:
         w = L.DecoderWeights(from_latent_w=t(weights["from_latent_w"]), from_latent_b=t(weights["from_latent_b"]),
                              output_w=t(weights["output_w"]), output_b=t(weights["output_b"]),
                              blocks=C.cast(blocks, C.POINTER(L.DecoderBlock)), num_blocks=len(weights["blocks"]))
-        self.ctx = _ctx(self.device)
+        self.ctx = _new_ctx(self.device)
         h = C.c_void_p()
         self.ctx.check(L.lib.p3d_decoder_create(self.ctx.h, C.byref(cfg), C.byref(w), C.byref(h)))
         self.h = h
@@ -81,7 +81,7 @@ class Decoder:
             stop_level: int | None = None):
         """Decode; returns (coords, feats, predicted subdivisions per level)
         or, with stop_level, the hidden (coords, feats) at that level."""
-        c = _ctx(self.device)
+        c = self.ctx.bind()
         stop = self.levels if stop_level is None else int(stop_level)
         gp = grows = None
         if guides is not None:

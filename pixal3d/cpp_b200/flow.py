@@ -16,7 +16,7 @@ import numpy as np
 import torch
 
 from . import _lib as L
-from .ops import ctx as _ctx
+from .ops import new_ctx as _new_ctx
 
 # reference field name -> p3d struct field
 TOP_MAP = {"input_weight": "input_w", "input_bias": "input_b", "timestep_weight0": "t_w0", "timestep_bias0": "t_b0",
@@ -105,7 +105,7 @@ class FlowModel:
                         setattr(arr[i], f, _ptr(t(rw[f])))
                 setattr(fw, side, C.cast(arr, C.POINTER(L.ResBlockWeights)))
                 io_arrays.append(arr)
-        self.ctx = _ctx(device)
+        self.ctx = _new_ctx(device)
         h = C.c_void_p()
         hpc = hp.to_c()
         self.ctx.check(L.OPTIONAL["p3d_flow_create"](self.ctx.h, C.byref(hpc), C.byref(fw), C.byref(h)))
@@ -118,13 +118,13 @@ class FlowModel:
         self.coords = coords
         self.batch = batch
         self.n = coords.shape[0]
-        self.ctx = _ctx(self.device)
+        self.ctx.bind()
         self.ctx.check(L.OPTIONAL["p3d_flow_prepare"](self.h, _ptr(coords), self.n, batch, *shape, offs))
         self.prepared = True
 
     def forward(self, x: torch.Tensor, timesteps: torch.Tensor, ctx_feats: torch.Tensor,
                 proj: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
-        c = _ctx(self.device)
+        c = self.ctx.bind()
         if out is None:
             out = torch.empty((self.n, self.hp.out_channels), dtype=torch.float32, device=x.device)
         dt = {torch.bfloat16: L.P3D_BF16, torch.float16: L.P3D_F16}.get(ctx_feats.dtype, L.P3D_F32)
@@ -139,7 +139,7 @@ class FlowModel:
         """In-place Euler/CFG integration of x (f32 [n/2, out_channels], the
         conditional rows).  concat (f32 [n/2, in - out]): the fixed concat
         condition appended to the state in every forward."""
-        c = _ctx(self.device)
+        c = self.ctx.bind()
         cfg = L.SamplerConfig(steps=steps, sigma_min=sigma_min, rescale_t=rescale_t,
                               guidance_strength=guidance_strength, guidance_rescale=guidance_rescale,
                               guidance_interval_min=guidance_interval[0], guidance_interval_max=guidance_interval[1],

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import threading
 
 import torch
 
@@ -20,19 +21,31 @@ try:
 except ImportError as e:
     raise ImportError("pixal3d/cpp_b200/_bind.so is not built for this torch; run `python -m pixal3d.cpp_b200.build`") from e
 
-_CTX: dict[int, "Context"] = {}
+_CTX: dict[int, "Context"] = {}  # a device's first context, whose fault flag and launch count the others share
+_CTX_LOCK = threading.Lock()
+_MINE = threading.local()        # this thread's contexts
 
 
 class Context:
-    """One p3d_ctx per device; its stream follows torch's current stream."""
+    """A p3d_ctx; its stream follows torch's current stream.  Each host thread,
+    and each flow and decoder, has its own (p3d_ctx_fork), so a call of one
+    thread never moves another's to its stream."""
 
-    def __init__(self, device: int):
+    def __init__(self, device: int, root: "Context | None" = None):
         h = C.c_void_p()
-        rc = L.lib.p3d_ctx_create(device, None, C.byref(h))
+        rc = L.lib.p3d_ctx_fork(root.h, None, C.byref(h)) if root else L.lib.p3d_ctx_create(device, None, C.byref(h))
         if rc != 0:
             raise P3DError(rc, f"p3d_ctx_create(device={device}) failed")
         self.h = h
         self.device = device
+        self.root = root
+
+    def __del__(self):
+        try:
+            if self.root is not None:
+                L.lib.p3d_ctx_destroy(self.h)
+        except Exception:
+            pass
 
     def bind(self) -> "Context":
         s = torch.cuda.current_stream(self.device).cuda_stream
@@ -48,26 +61,44 @@ class Context:
 
     @property
     def launches(self) -> int:
+        """Kernels launched on the device through all of its contexts."""
         return int(L.lib.p3d_ctx_launch_count(self.h))
 
 
-def ctx(device: torch.device | int | None = None) -> Context:
+def _index(device: torch.device | int | None) -> int:
     if device is None:
-        idx = torch.cuda.current_device()
-    elif isinstance(device, torch.device):
-        idx = device.index if device.index is not None else torch.cuda.current_device()
-    else:
-        idx = int(device)
-    if idx not in _CTX:
-        _CTX[idx] = Context(idx)
-    return _CTX[idx].bind()
+        return torch.cuda.current_device()
+    if isinstance(device, torch.device):
+        return device.index if device.index is not None else torch.cuda.current_device()
+    return int(device)
 
 
-def _context_handle(device: int) -> int:
-    return ctx(device).h.value
+def _root(idx: int) -> Context:
+    root = _CTX.get(idx)
+    if root is None:
+        with _CTX_LOCK:
+            root = _CTX.get(idx)
+            if root is None:
+                root = _CTX[idx] = Context(idx)
+    return root
 
 
-_bind.setup(_context_handle, P3DError)
+def new_ctx(device: torch.device | int | None = None) -> Context:
+    """A context of the caller's own, bound to the current stream."""
+    idx = _index(device)
+    return Context(idx, _root(idx)).bind()
+
+
+def ctx(device: torch.device | int | None = None) -> Context:
+    """The calling thread's context, bound to its current stream."""
+    idx = _index(device)
+    mine = _MINE.__dict__.get(idx)
+    if mine is None:
+        mine = _MINE.__dict__[idx] = Context(idx, _root(idx))
+    return mine.bind()
+
+
+_bind.setup(lambda device: _root(device).h.value, P3DError)
 
 
 def _need(ok: bool, message: str) -> None:
