@@ -16,10 +16,27 @@ import torch
 
 from . import _lib as L
 from ._lib import P3DError
+
+
+class _Unbuilt:
+    """Stands for _bind.so where it is not built for the installed torch: its
+    four operators fail when they are called, the others need it not."""
+
+    def __init__(self, cause: ImportError):
+        self._cause = cause
+
+    def setup(self, *args) -> None:
+        pass
+
+    def __getattr__(self, name: str):
+        raise ImportError(f"{name}: pixal3d/cpp_b200/_bind.so is not built for this torch; run `python -m pixal3d.cpp_b200.build`") \
+            from self._cause
+
+
 try:
     from . import _bind
 except ImportError as e:
-    raise ImportError("pixal3d/cpp_b200/_bind.so is not built for this torch; run `python -m pixal3d.cpp_b200.build`") from e
+    _bind = _Unbuilt(e)
 
 _CTX: dict[int, "Context"] = {}  # a device's first context, whose fault flag and launch count the others share
 _CTX_LOCK = threading.Lock()
