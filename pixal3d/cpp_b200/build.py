@@ -29,6 +29,7 @@ LIB = PKG / "libp3dcuda.so"
 HOST_LIB = PKG / "libpixal3d_b200.so"
 BIND = PKG / "bind" / "p3d_bind.cpp"
 BIND_LIB = PKG / "_bind.so"
+BIND_STAMP = BUILD / "bind.stamp"
 INCLUDE = REPO / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -99,17 +100,25 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
 
 
 def _build_bind(force: bool, verbose: bool) -> None:
-    """_bind.so: rebuilt when its source, the C header or torch itself changes."""
+    """_bind.so, where torch is installed: rebuilt when its source, the C header,
+    torch or Python change.  BIND_STAMP holds which torch and Python it is for, as
+    another one's files may be older."""
     import importlib.util
     import sysconfig
-    torch = Path(importlib.util.find_spec("torch").origin).parent
-    if not force and not _stale(BIND_LIB, BIND, [INCLUDE / "p3d.h", torch / "version.py"]):
+    spec = importlib.util.find_spec("torch")
+    if spec is None or spec.origin is None:
+        print("torch is not installed: the libraries are built without the torch binding", file=sys.stderr)
+        return
+    torch = Path(spec.origin).parent
+    stamp = f"{torch}\n{(torch / 'version.py').read_text()}\n{sys.version}\n"
+    if not force and not _stale(BIND_LIB, BIND, [INCLUDE / "p3d.h"]) and BIND_STAMP.exists() and BIND_STAMP.read_text() == stamp:
         return
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-I{INCLUDE}", f"-isystem{torch / 'include'}",
           f"-isystem{torch / 'include' / 'torch' / 'csrc' / 'api' / 'include'}", "-I/usr/local/cuda/include",
           f"-I{sysconfig.get_paths()['include']}", str(BIND), "-o", str(BIND_LIB), f"-L{PKG}", "-lp3dcuda",
           f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10",
           "-Wl,-rpath,$ORIGIN"], verbose)
+    BIND_STAMP.write_text(stamp)
 
 
 def main() -> None:
