@@ -115,8 +115,8 @@ int masked_attention_tiles(p3d_ctx *ctx, const MaskedParams &p, int head_dim, in
     return head_dim == 64 ? masked_tiles_f16_64(ctx, p, dtype) : masked_tiles_f16_128(ctx, p, dtype);
 }
 
-// Few queries over long keys: rows of an item (8, 16, 24 or 32 of the K/V
-// head's queries and heads), 16-key tiles of a piece, blocks, pieces at most,
+// Few queries over long keys: rows of an item (8 or 16 of the K/V head's
+// queries and heads), 16-key tiles of a piece, blocks, pieces at most,
 // and the bytes of their results.
 struct PiecePlan {
     int item_rows, piece, most_pieces, blocks;
@@ -124,8 +124,14 @@ struct PiecePlan {
     size_t o, ml;
     PiecePlan(int nseq, int64_t max_q, int64_t max_k, int64_t rows_k, int heads, int kv_heads, int head_dim) {
         const int64_t rows = std::max<int64_t>(max_q * (heads / kv_heads), 1);
-        // more rows of 128 dims would not stay in registers
-        item_rows = static_cast<int>(std::min<int64_t>(ceil_div(rows, 8) * 8, head_dim == 64 ? 32 : 16));
+        // More than 8 rows take passes of 16.  us by passes of at most 8 / 16 rows
+        // (sequences x queries, heads over K/V heads, keys a sequence), 64 dims:
+        // 4 x 8, 32 over 8, 16000 keys 79.4 / 66.6; 4 x 5, 16 over 4, 16000 34.6 /
+        // 36.0; 8 x 1, 32 over 1, 16000 26.9 / 21.9; 4 x 1, 24 over 1, 9000 13.0 /
+        // 14.8; 128 dims: 121.6 / 105.5, 51.9 / 56.0, 38.2 / 31.8, 16.3 / 18.8.
+        // Passes of 24 and 32 rows of 64 dims leave the registers: 73.6, 31.2, 28.9
+        // and 17.2.
+        item_rows = rows > 8 ? 16 : 8;
         const int64_t items = kv_heads * ceil_div(rows, item_rows);  // of a sequence
         const int64_t tiles = std::max<int64_t>(1, ceil_div(std::min(rows_k, nseq * max_k) / nseq, 16));  // of a mean item
         // The fewest rounds of the 148 blocks times a piece's length and its own
