@@ -23,6 +23,12 @@ constexpr int64_t kFewRows = 8, kFewKeys = 512;
 // short to matter.
 constexpr int kOrderTiles = 1024;
 
+// The SMs that work is cut for, B200's.  The plans below give the workspace's size
+// too, which is asked for without a context, so the size and the call must agree:
+// a context whose device has other SMs runs the same plan.
+constexpr int64_t kPlanSms = 148;
+constexpr int64_t kPlaces = 2 * kPlanSms;  // CTAs of masked_fmha_kernel at once
+
 size_t align256(size_t b) { return (b + 255) / 256 * 256; }
 
 // Smallest and largest document number of every key block, a warp a block.
@@ -134,24 +140,24 @@ struct PiecePlan {
         item_rows = rows > 8 ? 16 : 8;
         const int64_t items = kv_heads * ceil_div(rows, item_rows);  // of a sequence
         const int64_t tiles = std::max<int64_t>(1, ceil_div(std::min(rows_k, nseq * max_k) / nseq, 16));  // of a mean item
-        // The fewest rounds of the 148 blocks times a piece's length and its own
+        // The fewest rounds of the blocks, one an SM, times a piece's length and its own
         // cost, over pieces of whole stages and no longer than a block's even
         // share, so that uneven sequences end together (4 sequences of up to
         // 16000 keys, 5 queries 89 against 122 us without that bound; the own
         // cost taken as 8 tiles, not 32: 5 sequences of up to 16381 keys, 32
         // heads over 8 55.3 against 52.4 us).
-        const int64_t share = std::max<int64_t>(nseq * items * tiles / 148, 16);
+        const int64_t share = std::max<int64_t>(nseq * items * tiles / kPlanSms, 16);
         int64_t best = 0;
         piece = 16;
         for (int64_t l = 16; l < std::min(tiles, share) + 16; l += std::max<int64_t>(16, l / 8 / 16 * 16)) {
-            const int64_t cost = ceil_div(nseq * items * ceil_div(tiles, l), 148) * (l + 32);
+            const int64_t cost = ceil_div(nseq * items * ceil_div(tiles, l), kPlanSms) * (l + 32);
             if (best == 0 || cost < best) {
                 best = cost;
                 piece = static_cast<int>(l);
             }
         }
         most_pieces = static_cast<int>(ceil_div(std::max<int64_t>(max_k, 1), 16 * static_cast<int64_t>(piece)));
-        blocks = static_cast<int>(std::min<int64_t>(148, nseq * items * most_pieces));
+        blocks = static_cast<int>(std::min<int64_t>(kPlanSms, nseq * items * most_pieces));
         // of all sequences: by their number, or by the rows that they share
         parts = items * std::min(static_cast<int64_t>(nseq) * most_pieces, (rows_k / 16 + nseq) / piece + nseq);
         o = align256(static_cast<size_t>(parts) * item_rows * head_dim * sizeof(float));
@@ -160,7 +166,7 @@ struct PiecePlan {
 };
 
 // Many queries: splits of the key blocks (where the CTAs would fill less than
-// half of the GPU's 296 places, pieces of at least 8 blocks), whether the tiles
+// half of the GPU's places, pieces of at least 8 blocks), whether the tiles
 // are ordered (documents, more CTAs than places), and the bytes of the
 // documents' ranges, of the order and of the splits' results.
 struct TilePlan {
@@ -170,12 +176,12 @@ struct TilePlan {
     size_t docs, order, o, ml;
     TilePlan(int nseq, int64_t max_q, int64_t max_k, int64_t rows_k, int heads, int head_dim, bool documents) {
         const int64_t ctas = static_cast<int64_t>(heads) * nseq * ceil_div(max_q, 128);
-        splits = ctas > 148 ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({296 / std::max<int64_t>(ctas, 1), max_k / 512, 16})));
+        splits = ctas > kPlanSms ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kPlaces / std::max<int64_t>(ctas, 1), max_k / 512, 16})));
         tiles = nseq * ceil_div(max_q, 128);
-        ordered = documents && ctas > 296 && tiles <= kOrderTiles;
+        ordered = documents && ctas > kPlaces && tiles <= kOrderTiles;
         order = ordered ? align256(static_cast<size_t>(2 * tiles + 1) * sizeof(int4)) : 0;
         docs = documents ? align256(static_cast<size_t>(rows_k / 64 + nseq + 1) * sizeof(int2)) : 0;
-        // at most 296 x 128 rows, whatever rows q has beside the sequences'
+        // at most kPlaces x 128 rows, whatever rows q has beside the sequences'
         const size_t parts = splits > 1 ? static_cast<size_t>(nseq) * max_q * heads * splits : 0;
         o = align256(parts * head_dim * sizeof(float));
         ml = align256(parts * sizeof(float2));
