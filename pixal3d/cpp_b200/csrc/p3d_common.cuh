@@ -96,6 +96,12 @@ struct DeviceGuard {
                                     std::string(#expr ": ") + cudaGetErrorString(e_)); \
     } while (0)
 
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                              const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+// cuTensorMapEncodeTiled, or null where the driver lacks it (p3d_gemm.cu).
+EncodeFn get_encode_fn();
+
 // Encode a 2D 16-bit (bf16/f16) tensor map (rows x cols, row pitch in elements) with a
 // box of box_rows x 64 columns and 128-byte swizzle, the canonical K-major
 // SW128 operand layout of tcgen05.mma.
@@ -296,6 +302,15 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity
             return false;
         }
     }
+}
+
+// Warp-uniform bounded wait: lane 0 polls, the warp follows its verdict.
+template <bool CLUSTER>
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, int *fault) {
+    int ok = 1;
+    if ((threadIdx.x & 31) == 0)
+        ok = (CLUSTER ? mbar_wait_cluster(bar, parity, fault) : mbar_wait(bar, parity, fault)) ? 1 : 0;
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 __device__ __forceinline__ void tmem_alloc2(uint32_t *smem_result, uint32_t ncols) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_result)),

@@ -35,7 +35,7 @@
 #include <cstring>
 #include <mutex>
 
-#include "p3d_epilogue.cuh"
+#include "p3d_common.cuh"
 
 namespace p3d {
 
@@ -91,8 +91,10 @@ struct GemmParams {
     const uint32_t *tile_taps;
 };
 
-// TMA-store epilogue staging (p3d_epilogue.cuh): each epilogue warp owns one
-// or two slots.  EPI_BYTES: the 4 warps x 2 slots of the pair kernel.
+// TMA-store epilogue staging: each epilogue warp owns one or two 4 KB slots,
+// each one 32-row x 128-byte box (32 f32 or 64 16-bit columns) in the
+// 128-byte swizzle.  EPI_BYTES: the 4 warps x 2 slots of the pair kernel.
+constexpr int EPI_SLOT_BYTES = 4096;
 constexpr int EPI_WARP_BYTES = 2 * EPI_SLOT_BYTES;
 constexpr int EPI_BYTES = 4 * EPI_WARP_BYTES;
 
@@ -141,6 +143,25 @@ struct Cfg2 {
     static constexpr int TMEM_COLS = 512;
     static constexpr int SMEM = STAGES * STAGE_BYTES + EPI_BYTES + 1024 /*align*/ + 512 /*barriers*/;
 };
+
+template <typename T>
+__device__ __forceinline__ void store16(T *o, const float (&v)[32], int ncols) {
+    if (ncols == 32 && ((reinterpret_cast<uintptr_t>(o) & 15) == 0)) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+            uint4 pk;
+            pk.x = pack2<T>(v[i], v[i + 1]);
+            pk.y = pack2<T>(v[i + 2], v[i + 3]);
+            pk.z = pack2<T>(v[i + 4], v[i + 5]);
+            pk.w = pack2<T>(v[i + 6], v[i + 7]);
+            *reinterpret_cast<uint4 *>(o + i) = pk;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (i < ncols) o[i] = from_f32<T>(v[i]);
+    }
+}
 
 __device__ __forceinline__ void store_chunk(const GemmParams &p, int64_t row, int64_t col0, const float (&v)[32],
                                             int ncols) {
@@ -359,6 +380,58 @@ __device__ __forceinline__ void mul_vec32(float (&v)[32], const float *g, int nc
         for (int i = 0; i < 32; ++i)
             if (i < ncols) v[i] *= __ldg(g + i);
     }
+}
+
+// Staging slot for the next box: wait until the box last issued from this
+// slot (two boxes ago) has been read by the TMA unit.
+template <int SLOTS>
+__device__ __forceinline__ uint8_t *acquire_slot(uint8_t *wbuf, int slot, int lane) {
+    if (lane == 0) bulk_wait_read<SLOTS - 1>();
+    __syncwarp();
+    return wbuf + slot * EPI_SLOT_BYTES;
+}
+
+// This lane's 32 values as row `lane` of the slot, in the 128-byte swizzle
+// (16-byte chunk c of a 128-byte row at c ^ (row & 7)).  f32: the whole
+// 128-byte row; 16-bit: half `half` (columns 32*half .. +31) of a 64-column row.
+__device__ __forceinline__ void stage_row(int out_dtype, uint8_t *buf, int lane, const float (&v)[32], int half) {
+    uint8_t *rowp = buf + lane * 128;
+    if (out_dtype == P3D_F32) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            *reinterpret_cast<float4 *>(rowp + ((c ^ (lane & 7)) << 4)) =
+                make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+        return;
+    }
+    const bool bf = out_dtype == P3D_BF16;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        uint4 pk;
+        pk.x = bf ? pack2<__nv_bfloat16>(v[8 * c], v[8 * c + 1]) : pack2<__half>(v[8 * c], v[8 * c + 1]);
+        pk.y = bf ? pack2<__nv_bfloat16>(v[8 * c + 2], v[8 * c + 3]) : pack2<__half>(v[8 * c + 2], v[8 * c + 3]);
+        pk.z = bf ? pack2<__nv_bfloat16>(v[8 * c + 4], v[8 * c + 5]) : pack2<__half>(v[8 * c + 4], v[8 * c + 5]);
+        pk.w = bf ? pack2<__nv_bfloat16>(v[8 * c + 6], v[8 * c + 7]) : pack2<__half>(v[8 * c + 6], v[8 * c + 7]);
+        *reinterpret_cast<uint4 *>(rowp + (((4 * half + c) ^ (lane & 7)) << 4)) = pk;
+    }
+}
+
+// Lane 0 writes the staged 32-row box at (col0, row0): a TMA store, or (the
+// residual epilogue, or part of a tile cut by the split schedule) a TMA
+// reduce-add into the f32 output.  Rows >= M and columns >= N of the box are
+// clipped by the tensor map's bounds.
+template <int SLOTS>
+__device__ __forceinline__ void issue_box(const CUtensorMap *tmo, const uint8_t *buf, int lane, int64_t col0,
+                                          int64_t row0, int &slot, bool reduce) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+        if (reduce)
+            tma_reduce_add_2d(tmo, buf, static_cast<int>(col0), static_cast<int>(row0));
+        else
+            tma_store_2d(tmo, buf, static_cast<int>(col0), static_cast<int>(row0));
+        bulk_commit();
+    }
+    slot = SLOTS == 1 ? 0 : slot ^ 1;
 }
 
 // Bias (null: none), activation and residual gate of one 32-column chunk of
@@ -1345,6 +1418,29 @@ bool tma_out_ok(const GemmParams &p) {
            p.N < (int64_t(1) << 31);
 }
 
+// Output map for the TMA epilogue: [M rows, N cols] at pitch ldo, boxes of
+// 32 rows x 128 bytes (32 f32 or 64 16-bit columns) in the 128-byte swizzle,
+// matching the staging layout of stage_row.
+int make_tmap_out(p3d_ctx *ctx, CUtensorMap *map, void *base, int dtype, uint64_t rows, uint64_t cols, uint64_t ld) {
+    EncodeFn fn = get_encode_fn();
+    if (!fn) return set_error(ctx, P3D_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+    const bool f32 = dtype == P3D_F32;
+    const uint64_t es = f32 ? 4 : 2;
+    cuuint64_t dims[2] = {cols, rows};
+    cuuint64_t strides[1] = {ld * es};
+    cuuint32_t box[2] = {f32 ? 32u : 64u, 32};  // 128-byte box rows
+    cuuint32_t estr[2] = {1, 1};
+    const CUtensorMapDataType dt = f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                       : (dtype == P3D_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
+    CUresult r = fn(map, dt, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return set_error(ctx, P3D_ERR_CUDA, "cuTensorMapEncodeTiled (output) failed: " + std::to_string(r));
+    return P3D_OK;
+}
+
 // x == nullptr selects the gather (sparse conv) variant, whose B operand is
 // the [27 * N, K] tap stack.  Builds the tensor maps and instruction
 // descriptor for the chosen kernel and launches it.
@@ -1407,29 +1503,6 @@ EncodeFn get_encode_fn() {
             fn = reinterpret_cast<EncodeFn>(ptr);
     });
     return fn;
-}
-
-// Output map for the TMA epilogue: [M rows, N cols] at pitch ldo, boxes of
-// 32 rows x 128 bytes (32 f32 or 64 16-bit columns) in the 128-byte swizzle,
-// matching the staging layout of stage_row.
-int make_tmap_out(p3d_ctx *ctx, CUtensorMap *map, void *base, int dtype, uint64_t rows, uint64_t cols, uint64_t ld) {
-    EncodeFn fn = get_encode_fn();
-    if (!fn) return set_error(ctx, P3D_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
-    const bool f32 = dtype == P3D_F32;
-    const uint64_t es = f32 ? 4 : 2;
-    cuuint64_t dims[2] = {cols, rows};
-    cuuint64_t strides[1] = {ld * es};
-    cuuint32_t box[2] = {f32 ? 32u : 64u, 32};  // 128-byte box rows
-    cuuint32_t estr[2] = {1, 1};
-    const CUtensorMapDataType dt = f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                                       : (dtype == P3D_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
-    CUresult r = fn(map, dt, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
-                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS)
-        return set_error(ctx, P3D_ERR_CUDA, "cuTensorMapEncodeTiled (output) failed: " + std::to_string(r));
-    return P3D_OK;
 }
 
 int make_tmap_16bit_2d(p3d_ctx *ctx, CUtensorMap *map, const void *base, int dtype, uint64_t rows, uint64_t cols,

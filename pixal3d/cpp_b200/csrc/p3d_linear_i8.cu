@@ -28,7 +28,7 @@
 #include <algorithm>
 #include <cstring>
 
-#include "p3d_epilogue.cuh"
+#include "p3d_common.cuh"
 
 namespace p3d {
 namespace {
