@@ -330,7 +330,8 @@ int p3d_varlen_attention(p3d_ctx *ctx, const void *q, int64_t ldq, const void *k
 
 /* Rules of p3d_masked_attention; zeros and NULLs mean none. */
 typedef struct p3d_attention_rules {
-    float softcap;         /* 1e-6 .. 1e6: scores become softcap * tanh(score / softcap); 0: none */
+    float softcap;         /* 1e-6 .. 1e6: scores become softcap * tanh(score / softcap), to 2^-22 of the
+                              cap, near ones (within half the cap) to 2^-18 of themselves; 0: none */
     int causal;            /* nonzero: a query sees the keys up to its own position */
     const int32_t *prefix; /* [nseq]: the first prefix[s] keys of sequence s are seen by all its queries */
     const int32_t *doc_q;  /* [rows_q] and [rows_k], both or none: a query sees the keys of its own */
@@ -346,11 +347,14 @@ typedef struct p3d_attention_rules {
  *   j < prefix[s], or (not causal or j <= position) and the documents agree.
  * A query that sees no key gets zeros.  What hidden keys and rows outside the
  * sequences hold (NaN, infinities) never reaches an output; rows of out
- * outside the sequences are left as they were.
+ * outside the sequences are left as they were.  For sequences without any rule,
+ * one head a K/V head, head_dim 64 and many queries p3d_varlen_attention is some
+ * 8 % faster, with weights from 16-bit exponents (1 % of a weight).
  * q [rows_q][ldq], out [rows_q][ldo]: heads * head_dim columns; k, v
  * [rows_k][ldk / ldv]: kv_heads * head_dim columns, query head h reads
  * key/value head h / (heads / kv_heads).  head_dim 64 or 128, dtype bf16 or
- * f16, f32 softmax and accumulation, 16-byte aligned rows.  max_q / max_k
+ * f16, f32 softmax and accumulation, the weights rounded to dtype for their
+ * product with v and summed as rounded, 16-byte aligned rows.  max_q / max_k
  * bound the queries / keys of one sequence (queries from max_q on are not
  * computed; a max_k below the longest sequence costs time only).  The two offset arrays
  * are device data and are clamped to the row counts.  ws:

@@ -6,7 +6,7 @@
 // 2^31); it is rounded once to f32 (24 bits), then scaled in f32.
 //
 // More than a few rows run on the tensor cores (tcgen05.mma kind::i8, 32-bit
-// integer accumulators in TMEM).  CTA = 10 warps, persistent over the tiles:
+// integer accumulators in TMEM).  CTA = 18 warps, persistent over the tiles:
 //   warps 0-15  epilogue: four per TMEM lane quarter, each its share of the
 //               columns; lane = row; scales, bias, activation, then boxes of
 //               32 rows x 64 bytes staged in shared memory and written by TMA

@@ -186,7 +186,7 @@ __device__ __forceinline__ void bias_row(float (&s)[64], float scale, float slop
     const float df = static_cast<float>(d);
     const bool left = __all_sync(0xffffffffu, d >= 63), right = __all_sync(0xffffffffu, d <= 0);
     if (left || right) {
-        const float step = left ? slope : -slope, base = -step * df;  // exact sign; one rounding, as in the other form
+        const float step = left ? slope : -slope, base = -step * df;  // its rounding, 2^-24 of slope d, is the one that the other form lacks
 #pragma unroll
         for (int e = 0; e < 64; e += 2)
             fma2(F2(s[e], s[e + 1]), F2(scale, scale),

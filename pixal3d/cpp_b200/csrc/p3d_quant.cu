@@ -20,7 +20,7 @@
 // takes about five instructions.  A row is read in the 16-byte words it
 // touches, wherever it starts: a word never crosses an allocation, and what
 // lies beside the row is masked.  8184 x 4096 f16 takes
-// 18.4 us (5.5 TB/s), f32 27.4 (6.1 TB/s).
+// 18.2 us (5.5 TB/s), f32 27.2 (6.2 TB/s).
 #include "p3d_common.cuh"
 
 namespace p3d {
