@@ -26,6 +26,8 @@ Kernels (config-2 shapes unless noted):
   euler      Euler/CFG update with guidance rescale, 21,766 x 8
   qrows      row quantisation to 8-bit integers, 8,184 x 4096 f16
   lin8       trunk MLP up-projection with GELU on 8-bit integers, 8,184 x 1024 -> 4096
+  lin8r      trunk out-projection on 8-bit integers, gated residual into f32, 8,184 x 1024 -> 1024
+  lin8few    modulation of two items on 8-bit integers, 2 x 1024 -> 6144
   rotary     rotary positions, 16,368 rows x 32 heads x 64, interleaved, f16
   mattn      masked attention, 2 x 4,092 rows, 16 heads x 64, causal behind 1,029 prefix keys, scores capped
   mtoken     masked attention of one token of 5 sequences of 16,381 keys, 32 heads x 128 over 8
@@ -287,6 +289,22 @@ def run(kernel: str, reps: int, chunk: int | None = None) -> dict:
         out = torch.empty((m, n), dtype=torch.bfloat16, device=dev)
         ms = _time(lambda: ops.linear_i8(x, xs, w, ws, b, out=out, epilogue=L.EPI_GELU_TANH), reps)
         return {"kernel": kernel, "ms": ms, "tops": 2.0 * m * n * k / ms / 1e9}
+    if kernel == "lin8r":
+        m = 8184
+        x, xs = ops.quantize_rows(torch.randn((m, C), device=dev, generator=g))
+        w, ws = ops.quantize_rows(torch.randn((C, C), device=dev, generator=g) / math.sqrt(C))
+        b, gate = torch.zeros(C, device=dev), torch.ones((2, C), device=dev)
+        off = torch.tensor([0, m // 2, m], dtype=torch.int32, device=dev)
+        out = torch.zeros((m, C), device=dev)
+        ms = _time(lambda: ops.linear_i8(x, xs, w, ws, b, out=out, epilogue=L.EPI_RESIDUAL, gate=gate, batch_offsets=off), reps)
+        return {"kernel": kernel, "ms": ms, "tops": 2.0 * m * C * C / ms / 1e9}
+    if kernel == "lin8few":
+        m, n = 2, 6 * C
+        x, xs = ops.quantize_rows(torch.randn((m, C), device=dev, generator=g))
+        w, ws = ops.quantize_rows(torch.randn((n, C), device=dev, generator=g) / math.sqrt(C))
+        b, out = torch.zeros(n, device=dev), torch.empty((m, n), device=dev)
+        ms = _time(lambda: ops.linear_i8(x, xs, w, ws, b, out=out), reps)
+        return {"kernel": kernel, "ms": ms, "gbs": n * C / ms / 1e6}
     if kernel == "rotary":
         n, heads = 16368, 32
         x = torch.randn((n, heads * 64), device=dev, generator=g).to(h)

@@ -381,7 +381,9 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     seen when j < prefix[s], or (not causal or j <= the query's position) and
     doc_k equals doc_q; scores are softcap * tanh(score / softcap) -
     slopes[head] * |position - j|.  A query that sees nothing gets zeros; rows
-    of a new out behind the last sequence are not written."""
+    of a new out behind the last sequence are not written.  One kernel takes
+    the whole call, by max_q: single tokens over long keys are faster without a
+    prompt beside them."""
     return _bind.masked_attention(q, k, v, cu_q, cu_k, max_q, max_k, heads, scale, kv_heads, causal, prefix, doc_q, doc_k, slopes,
                                   softcap, out)
 
