@@ -464,7 +464,8 @@ __global__ void __launch_bounds__(kThreadsF, 2)
         auto visible = [&](int j) -> bool {
             return j < edge && (j < pre || !DOCS || ((!p.causal || j <= pos) && p.doc_k[sr.k0 + j] == docq));
         };
-        const NearCap near(p.c0, p.c1);
+        NearCap near(p.c0, p.c1);
+        if (!valid) near.top = INFINITY;  // a row past the end has no say: what it holds changes no output's rounding
         float m_run = -INFINITY;
         float l0 = 0.0f, l1 = 0.0f;  // 128 dims: the sum of weights, even and odd keys
         bool ok = true;
@@ -530,7 +531,7 @@ __global__ void __launch_bounds__(kThreadsF, 2)
                 if constexpr (CAP && !BIAS) {
                     if (all) {
                         mx = row_max64(s);
-                        folded = __all_sync(0xffffffffu, fmaxf(mx, -row_min64(s)) <= near.top);
+                        folded = __all_sync(0xffffffffu, !(fmaxf(mx, -row_min64(s)) > near.top));
                         const float u = mx * mx;
                         mx *= fmaf(fmaf(fmaf(u, near.f3, near.f2), u, near.f1), u, near.f0);
                     }

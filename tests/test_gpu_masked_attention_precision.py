@@ -114,3 +114,32 @@ def test_values_that_are_alike_average_to_themselves(lq, n, d, dtype, rules):
     got = o.masked_attention(q, k, v, cu([lq]), cu([n]), lq, n, 2, 1.0, **rules)
     o.ctx().sync_check()
     assert torch.equal(got, v[:1].expand_as(got)), float((got.double() / v[0].double() - 1).abs().max())
+
+
+@pytest.mark.parametrize("softcap", [0.0, 20.0])
+@pytest.mark.parametrize("d,dtype", [(64, HF), (64, BF), (128, HF), (128, BF)])
+@pytest.mark.parametrize("lens", [[(200, 200)], [(70, 900), (5, 5)], [(300, 4000)], [(3, 700), (8, 900)], [(2, 100)]])
+def test_what_lies_beside_changes_no_bit(lens, d, dtype, softcap):
+    """Rows behind the last sequence and hidden keys may hold anything: the same
+    outputs to the last bit."""
+    o = ops()
+    g = torch.Generator(device="cuda").manual_seed(23)
+    nq, nk = sum(a for a, _ in lens), sum(b for _, b in lens)
+    q = torch.randn((nq + 140, 2 * d), device="cuda", generator=g).to(dtype)
+    k, v = (torch.randn((nk + 140, 2 * d), device="cuda", generator=g).to(dtype) for _ in range(2))
+    cq, ck = cu([a for a, _ in lens]), cu([b for _, b in lens])
+    doc = torch.zeros(nk + 140, dtype=torch.int32, device="cuda")
+    doc[7:nk // 2:11] = 99
+    dq = torch.zeros(nq + 140, dtype=torch.int32, device="cuda")
+    hidden = (doc == 99).nonzero().flatten()
+    for rules in (dict(), dict(causal=True), dict(doc_q=dq, doc_k=doc)):
+        got = []
+        for value in (0.0, 3e4, math.inf, math.nan):
+            for t in (q[nq:], k[nk:], v[nk:]):
+                t.fill_(value)
+            if "doc_q" in rules:
+                k[hidden] = v[hidden] = value
+            out = o.masked_attention(q, k, v, cq, ck, max(a for a, _ in lens), max(b for _, b in lens), 2, 0.2, softcap=softcap, **rules)
+            got.append(out[:nq])
+        o.ctx().sync_check()
+        assert all(torch.equal(got[0], x) for x in got[1:]), (rules.keys(), [int((got[0] != x).sum()) for x in got])
