@@ -544,3 +544,18 @@ def test_sequences_longer_than_max_k(d, dtype):
         got = o.masked_attention(q, k, v, cu([a for a, _ in lens]), cu([b for _, b in lens]), 3, max_k, 8, 0.1, kv_heads=2, causal=True)
         o.ctx().sync_check()
         assert bool(((got.double() - want).abs() <= tol).all()), max_k
+
+
+@pytest.mark.parametrize("extra", [(1, 1), (1, 600), (9, 20)])
+def test_the_most_sequences(extra):
+    """65535 sequences, all but one of a single query and key: its value."""
+    o = ops()
+    n, d = 65534, 64
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q, k, v = (torch.randn((n + e, d), device="cuda", generator=g).half() for e in (extra[0], extra[1], extra[1]))
+    at = [torch.cat([torch.arange(n + 1), torch.tensor([n + e])]).int().cuda() for e in extra]
+    got = o.masked_attention(q, k, v, at[0], at[1], extra[0], extra[1], 1, 0.125)
+    o.ctx().sync_check()
+    assert torch.equal(got[:n], v[:n])
+    want, tol = attention64(q[n:], k[n:], v[n:], [extra], 1, 1, 0.125)
+    assert bool(((got[n:].double() - want).abs() <= tol).all())
