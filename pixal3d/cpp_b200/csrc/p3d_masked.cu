@@ -121,7 +121,7 @@ int masked_attention_tiles(p3d_ctx *ctx, const MaskedParams &p, int head_dim, in
     return head_dim == 64 ? masked_tiles_f16_64(ctx, p, dtype) : masked_tiles_f16_128(ctx, p, dtype);
 }
 
-// Few queries over long keys: rows of an item (8 or 16 of the K/V head's
+// Few queries over long keys: rows of an item (8, 16 or 24 of the K/V head's
 // queries and heads), 16-key tiles of a piece, blocks, pieces at most,
 // and the bytes of their results.
 struct PiecePlan {
@@ -130,16 +130,18 @@ struct PiecePlan {
     size_t o, ml;
     PiecePlan(int nseq, int64_t max_q, int64_t max_k, int64_t rows_k, int heads, int kv_heads, int head_dim) {
         const int64_t rows = std::max<int64_t>(max_q * (heads / kv_heads), 1);
-        // More than 8 rows take passes of 16.  us by passes of at most 8 / 16 rows
-        // (sequences x queries, heads over K/V heads, keys a sequence), 64 dims:
-        // 4 x 8, 32 over 8, 16000 keys 79.4 / 66.6; 4 x 5, 16 over 4, 16000 34.6 /
-        // 36.0; 8 x 1, 32 over 1, 16000 26.9 / 21.9; 4 x 1, 24 over 1, 9000 13.0 /
-        // 14.8; 128 dims: 121.6 / 105.5, 51.9 / 56.0, 38.2 / 31.8, 16.3 / 18.8.
-        // Passes of 24 and 32 rows of 64 dims leave the registers: 73.6, 31.2, 28.9
-        // and 17.2.
-        item_rows = rows > 8 ? 16 : 8;
-        const int64_t items = kv_heads * ceil_div(rows, item_rows);  // of a sequence
         const int64_t tiles = std::max<int64_t>(1, ceil_div(std::min(rows_k, nseq * max_k) / nseq, 16));  // of a mean item
+        // Passes of 8 rows for up to 8, else of 16, but of 24 for 17 to 24 rows of 64
+        // dims (192 bytes of spills) over many keys, which then come once, not twice.
+        // us by passes of at most 16 / 24 (queries x heads of each K/V head x K/V
+        // heads, sequences x keys): 1 x 24 x 1, 16 x 9000 26.8 / 24.0; 5 x 4 x 4, 4 x
+        // 16000 36.0 / 31.2; 3 x 8 x 4, 2 x 16000 21.8 / 23.8; 6 x 4 x 4, 1 x 4000 11.0 /
+        // 13.5; 40 and 48 rows 20.0 / 23.4 and 29.2 / 39.8.  Of 8 / 16: 32 rows 26.9 / 21.9
+        // and 79.4 / 66.6, 128 dims 121.6 / 105.5 and 38.2 / 31.8 (20 rows 51.9 / 56.0).
+        // Passes of 32 rows (516 bytes) 28.9 and 73.6 instead of 21.9 and 66.6.
+        const bool once = head_dim == 64 && rows > 16 && rows <= 24 && nseq * kv_heads * tiles >= 8500;
+        item_rows = once ? 24 : rows > 8 ? 16 : 8;
+        const int64_t items = kv_heads * ceil_div(rows, item_rows);  // of a sequence
         // The fewest rounds of the blocks, one an SM, times a piece's length and its own
         // cost, over pieces of whole stages and no longer than a block's even
         // share, so that uneven sequences end together (4 sequences of up to

@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(kThreadsF, 2)
 #pragma unroll
                 for (int kk = 0; kk < kN / 16; ++kk)  // 16 keys: 8 packed TMEM columns of P, 2048 bytes of V
                     umma_f16_ts(tmem + kOCol, tmem + b * kN + kk * 8, sw128_desc_mn(v_addr + kk * 2048, next), idesc_o,
-                            (i > 0 || kk > 0) ? 1u : 0u);
+                                (i > 0 || kk > 0) ? 1u : 0u);
                 umma_commit(&pv_done[b]);
                 umma_commit(&v_empty[st]);
                 return true;

@@ -567,6 +567,9 @@ int launch_pieces(p3d_ctx *ctx, const MaskedParams &p, int dtype) {
 template <typename T, int D>
 int launch_rows(p3d_ctx *ctx, const MaskedParams &p, int dtype) {
     if (p.item_rows == 8) return launch_pieces<T, D, 1>(ctx, p, dtype);
+    if constexpr (D == 64) {
+        if (p.item_rows == 24) return launch_pieces<T, D, 3>(ctx, p, dtype);
+    }
     return launch_pieces<T, D, 2>(ctx, p, dtype);
 }
 

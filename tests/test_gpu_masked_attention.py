@@ -559,3 +559,10 @@ def test_the_most_sequences(extra):
     assert torch.equal(got[:n], v[:n])
     want, tol = attention64(q[n:], k[n:], v[n:], [extra], 1, 1, 0.125)
     assert bool(((got[n:].double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", [HF, BF])
+@pytest.mark.parametrize("lens,heads,kv_heads", [([(5, 12000)] * 3, 16, 4), ([(1, 9000)] * 16, 24, 1), ([(6, 44000), (2, 3000), (0, 7)], 12, 3)])
+def test_passes_of_24_rows(lens, heads, kv_heads, dtype):
+    """17 to 24 rows a K/V head over many keys: one pass over them."""
+    run(lens, heads, kv_heads, 64, dtype, causal=True, softcap=30.0)
